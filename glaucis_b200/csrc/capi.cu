@@ -60,6 +60,13 @@ int gl_launch_tgmm_fp8(const void* lq, const float* ls, const void* dq, const fl
                        const int32_t* group_sizes, int64_t G, int64_t M, int64_t K, int64_t N,
                        void* out, int out_f32, int* err, cudaStream_t st, int num_sms,
                        const char** why);
+int gl_launch_rms_norm_fwd(const void* x, const void* residual, const void* weight, int w32, float eps,
+                           int64_t M, int64_t K, void* h, void* y, void* q, float* s, float* rstd,
+                           cudaStream_t st, const char** why);
+size_t gl_rms_norm_bwd_ws_bytes(int64_t M, int64_t K, int num_sms);
+int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int w32,
+                           const float* rstd, int64_t M, int64_t K, void* dx, void* dw, void* ws,
+                           cudaStream_t st, int num_sms, const char** why);
 
 namespace {
 
@@ -624,6 +631,68 @@ int gl_tgmm_fp8(const void* lq, const float* ls, const void* dq, const float* ds
                                     static_cast<cudaStream_t>(stream), d->num_sms, &why);
   if (rc == -1) return fail(GL_EINVAL, std::string("gl_tgmm_fp8: ") + why);
   if (rc != 0) return fail(GL_ELAUNCH, std::string("gl_tgmm_fp8: ") + why);
+  return GL_OK;
+}
+
+static bool rms_norm_shape_ok(int64_t M, int64_t K) {
+  return M >= 0 && M <= 0x7fffffff && K > 0 && K <= GL_RMS_NORM_MAX_K && K % 8 == 0;
+}
+
+int gl_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_f32, float eps,
+                    int64_t M, int64_t K, void* h, void* y, void* q, float* s, float* rstd,
+                    int* err_word, void* stream) {
+  (void)err_word;
+  const char* f = "gl_rms_norm_fwd";
+  if (!rms_norm_shape_ok(M, K))
+    return fail(GL_EINVAL, std::string(f) + ": need 0 <= M < 2^31 and K a multiple of 8 in 8..16384");
+  if (M == 0) return GL_OK;  // empty tensors have no address to check
+  if (!x || !weight) return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if ((residual != nullptr) != (h != nullptr))
+    return fail(GL_EINVAL, std::string(f) + ": h goes with a residual (both or neither)");
+  if ((q != nullptr) != (s != nullptr)) return fail(GL_EINVAL, std::string(f) + ": q and s go together");
+  if (!y && !q) return fail(GL_EINVAL, std::string(f) + ": neither y nor q / s is asked for");
+  if (q && K % 128 != 0) return fail(GL_EINVAL, std::string(f) + ": q and s need K a multiple of 128");
+  if (!(eps >= 0.0f)) return fail(GL_EINVAL, std::string(f) + ": eps must be >= 0");
+  if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(h) || !aligned16(y) ||
+      !aligned16(q))
+    return fail(GL_EINVAL, std::string(f) + ": tensors must be 16-byte aligned");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_rms_norm_fwd(x, residual, weight, weight_f32 != 0, eps, M, K, h, y, q, s, rstd,
+                                        static_cast<cudaStream_t>(stream), &why);
+  if (rc != 0) return fail(rc == -1 ? GL_EINVAL : GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+size_t gl_rms_norm_bwd_workspace_bytes(int64_t M, int64_t K) {
+  if (!rms_norm_shape_ok(M, K) || M == 0) return 0;
+  DeviceState* d = nullptr;
+  if (device_state(&d)) return 0;
+  return gl_rms_norm_bwd_ws_bytes(M, K, d->num_sms);
+}
+
+int gl_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int weight_f32,
+                    const float* rstd, int64_t M, int64_t K, void* dx, void* dweight, void* workspace,
+                    size_t workspace_bytes, int* err_word, void* stream) {
+  (void)err_word;
+  const char* f = "gl_rms_norm_bwd";
+  if (!weight || !dweight || (M != 0 && (!dy || !h || !rstd || !dx)))
+    return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (!rms_norm_shape_ok(M, K))
+    return fail(GL_EINVAL, std::string(f) + ": need 0 <= M < 2^31 and K a multiple of 8 in 8..16384");
+  if (!aligned16(dy) || !aligned16(dh) || !aligned16(h) || !aligned16(weight) || !aligned16(dx) ||
+      !aligned16(dweight) || !aligned16(workspace))
+    return fail(GL_EINVAL, std::string(f) + ": tensors must be 16-byte aligned");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  if (M > 0 && (!workspace || workspace_bytes < gl_rms_norm_bwd_ws_bytes(M, K, d->num_sms)))
+    return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
+                                            "gl_rms_norm_bwd_workspace_bytes gives");
+  const char* why = "";
+  const int rc = gl_launch_rms_norm_bwd(dy, dh, h, weight, weight_f32 != 0, rstd, M, K, dx, dweight,
+                                        workspace, static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(rc == -1 ? GL_EINVAL : GL_ELAUNCH, std::string(f) + ": " + why);
   return GL_OK;
 }
 

@@ -30,13 +30,6 @@
 
 namespace gl {
 
-__device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  // The first source lands in the upper byte, the second in the lower byte.
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // Division by a block scale.  With y = RN(1/s) (one IEEE division per
 // block), q = RN(x*y) lies within one ulp of x/s, the residual r = x - q*s is
 // exact in one FMA, and RN(q + r*y) is the correctly rounded quotient
@@ -63,10 +56,6 @@ struct BlockDiv {
     fast = scale >= 0x1p-64f && scale <= 3.40282347e38f;
   }
 };
-
-__device__ __forceinline__ float2 bf16x2_to_f32x2(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
 
 // The two bf16 values of w as negated floats (sign bit flipped in the same
 // integer operation that widens them).

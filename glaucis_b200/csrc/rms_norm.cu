@@ -1,0 +1,366 @@
+// RMS norm with the residual's addition, forward and backward.
+//
+//   h = bf16(x + residual)            (h = x without a residual)
+//   r = 1 / sqrt(mean_k h^2 + eps),   y = h * r * w
+// out: y in bf16 and / or, per 128 features, the e4m3 pair of the activation
+// quantiser (s = max|y| / 448, 1 for an all-zero block; q = e4m3(y / s)),
+// quantised from y in 32 bits: the 8-bit output is rounded once, not first to
+// bf16.  The norm is that of the stored (rounded) h, so the backward pass,
+// which starts from h, differentiates exactly what ran forward.
+//   backward, u = w * dy, xh = h * r:
+//   dx = r * (u - xh * mean_k(u * xh)) + dh,   dw = sum_rows dy * xh
+//
+// Both passes are bound by HBM: a row is read once, held in registers as
+// 16-byte vectors (8 features a thread and vector) and written once.  The row
+// sums are held in 32 bits and reduced in a fixed order.
+#include "common.cuh"
+
+namespace gl {
+namespace rms {
+
+constexpr int MAX_K = 16384;  // 1024 threads x 2 vectors x 8 features
+constexpr int WARP_ROWS = 8;  // rows of a CTA when a warp takes a row
+
+struct FwdArgs {
+  const uint4* x;
+  const uint4* res;   // or null
+  const void* w;
+  uint4* h;           // with res
+  uint4* y;           // or null
+  uint2* q;           // or null
+  float* s;           // with q
+  float* rstd;        // or null
+  int64_t M;
+  int nvec;           // K / 8
+  int w32;
+  float inv_k, eps;
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = bf16x2_to_f32x2(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                    pack_bf16x2(f[6], f[7]));
+}
+
+__device__ __forceinline__ void load_w8(const void* w, int w32, int vec, float (&f)[8]) {
+  if (w32) {
+    const float4 a = __ldg(static_cast<const float4*>(w) + 2 * vec);
+    const float4 b = __ldg(static_cast<const float4*>(w) + 2 * vec + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    unpack8(__ldg(static_cast<const uint4*>(w) + vec), f);
+  }
+}
+
+// Sum over the threads of a row: a warp's own when a warp takes a row, else
+// over the CTA's warps through `part` (one slot per warp).
+template <bool kWarpRow>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+  v = warp_sum(v);
+  if (kWarpRow) return v;
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  if (lane == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return warp_sum(lane < nw ? part[lane] : 0.0f);
+}
+
+// V vectors a thread.  kWarpRow: a warp per row, WARP_ROWS rows a CTA; else a
+// CTA per row.
+template <int V, bool kWarpRow>
+__global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
+    rms_norm_fwd_kernel(const FwdArgs a) {
+  __shared__ float part[32];
+  const int64_t row = kWarpRow ? static_cast<int64_t>(blockIdx.x) * WARP_ROWS + (threadIdx.x >> 5)
+                               : static_cast<int64_t>(blockIdx.x);
+  if (kWarpRow && row >= a.M) return;
+  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
+  const int step = kWarpRow ? 32 : blockDim.x;
+  const int64_t base = row * a.nvec;
+
+  // plain loads: h may be x's or the residual's own buffer (every element is
+  // read before the same thread writes it)
+  uint4 xv[V], rv[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int vec = tid + i * step;
+    xv[i] = vec < a.nvec ? a.x[base + vec] : make_uint4(0, 0, 0, 0);
+    if (a.res) rv[i] = vec < a.nvec ? a.res[base + vec] : make_uint4(0, 0, 0, 0);
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int vec = tid + i * step;
+    float f[8];
+    unpack8(xv[i], f);
+    if (a.res) {
+      float g[8];
+      unpack8(rv[i], g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] += g[j];
+      xv[i] = pack8(f);  // the sum as it is stored: the one rounding of h
+      if (vec < a.nvec) a.h[base + vec] = xv[i];
+      unpack8(xv[i], f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
+  }
+  sum = row_sum<kWarpRow>(sum, part);
+  const float r = rsqrtf(fmaf(sum, a.inv_k, a.eps));
+  if (a.rstd && tid == 0) a.rstd[row] = r;
+
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int vec = tid + i * step;
+    float f[8], w[8];
+    if (vec < a.nvec) {
+      unpack8(xv[i], f);
+      load_w8(a.w, a.w32, vec, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
+      if (a.y) a.y[base + vec] = pack8(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+    }
+    if (a.q) {
+      // a block of 128 features is a half-warp's vectors (nvec % 16 == 0, so
+      // a half-warp is inside the row or past it as a whole)
+      float m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      const float s = m == 0.0f ? 1.0f : m / 448.0f;
+      if (vec < a.nvec) {
+        // one division per block; blocks whose reciprocal would overflow (or
+        // whose maximum is infinite) divide each element
+        if (s >= 0x1p-100f && s <= 3.40282347e38f) {
+          const float inv = 1.0f / s;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] *= inv;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] /= s;
+        }
+        uint32_t p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = cvt_e4m3x2(f[2 * j], f[2 * j + 1]);
+        a.q[base + vec] = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+        if ((tid & 15) == 0) a.s[row * (a.nvec >> 4) + (vec >> 4)] = s;
+      }
+    }
+  }
+}
+
+struct BwdArgs {
+  const uint4* dy;
+  const uint4* dh;    // or null
+  const uint4* h;
+  const void* w;
+  const float* rstd;
+  uint4* dx;
+  float* part;        // fp32 [gridDim.x, K]: each CTA's share of dw
+  int64_t M;
+  int nvec;
+  int w32;
+  float inv_k;
+};
+
+// A persistent CTA takes rows blockIdx.x, + gridDim.x, ... (kWarpRow: a warp
+// each) and keeps its columns' share of dw in registers.
+template <int V, bool kWarpRow>
+__global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
+    rms_norm_bwd_kernel(const BwdArgs a) {
+  __shared__ float part[2][32];
+  __shared__ float cross[kWarpRow ? WARP_ROWS : 1][kWarpRow ? 32 * V * 8 : 1];
+  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
+  const int step = kWarpRow ? 32 : blockDim.x;
+  const int64_t rows_step = kWarpRow ? static_cast<int64_t>(gridDim.x) * WARP_ROWS : gridDim.x;
+  int64_t row = kWarpRow ? static_cast<int64_t>(blockIdx.x) * WARP_ROWS + (threadIdx.x >> 5)
+                         : static_cast<int64_t>(blockIdx.x);
+  float dw[V][8] = {};
+  for (int it = 0; row < a.M; row += rows_step, it ^= 1) {
+    const int64_t base = row * a.nvec;
+    const float r = __ldg(a.rstd + row);
+    uint4 gv[V], hv[V], dv[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int vec = tid + i * step;
+      const bool in = vec < a.nvec;
+      gv[i] = in ? __ldg(a.dy + base + vec) : make_uint4(0, 0, 0, 0);
+      hv[i] = in ? __ldg(a.h + base + vec) : make_uint4(0, 0, 0, 0);
+      dv[i] = in && a.dh ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
+    }
+    float c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int vec = tid + i * step;
+      if (vec < a.nvec) {
+        float g[8], h[8], w[8];
+        unpack8(gv[i], g);
+        unpack8(hv[i], h);
+        load_w8(a.w, a.w32, vec, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float xh = h[j] * r;
+          c = fmaf(g[j] * w[j], xh, c);
+          dw[i][j] = fmaf(g[j], xh, dw[i][j]);
+        }
+      }
+    }
+    // two sets of slots: a warp may reach the next row's sum while another
+    // still reads this one's
+    c = row_sum<kWarpRow>(c, part[it]) * a.inv_k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int vec = tid + i * step;
+      if (vec < a.nvec) {
+        float g[8], h[8], d[8], w[8];
+        unpack8(gv[i], g);
+        unpack8(hv[i], h);
+        unpack8(dv[i], d);
+        load_w8(a.w, a.w32, vec, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = fmaf(r, fmaf(-h[j] * r, c, g[j] * w[j]), d[j]);
+        a.dx[base + vec] = pack8(d);
+      }
+    }
+  }
+  float* out = a.part + static_cast<int64_t>(blockIdx.x) * a.nvec * 8;
+  if (kWarpRow) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cross[threadIdx.x >> 5][(tid + i * 32) * 8 + j] = dw[i][j];
+    __syncthreads();
+    for (int k = threadIdx.x; k < a.nvec * 8; k += blockDim.x) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < WARP_ROWS; ++i) s += cross[i][k];
+      out[k] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int vec = tid + i * step;
+      if (vec < a.nvec) {
+        reinterpret_cast<float4*>(out)[2 * vec] = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
+        reinterpret_cast<float4*>(out)[2 * vec + 1] = make_float4(dw[i][4], dw[i][5], dw[i][6], dw[i][7]);
+      }
+    }
+  }
+}
+
+// dw[k] = sum over the CTAs' shares, in a fixed order.  32 columns x 32 row
+// lanes a CTA.
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, int n, int K, int w32,
+                                                           void* dw) {
+  __shared__ float sh[32][33];
+  const int k = blockIdx.x * 32 + (threadIdx.x & 31), rl = threadIdx.x >> 5;
+  float s = 0.0f;
+  if (k < K)
+    for (int i = rl; i < n; i += 32) s += __ldg(part + static_cast<int64_t>(i) * K + k);
+  sh[rl][threadIdx.x & 31] = s;
+  __syncthreads();
+  s = warp_sum(sh[threadIdx.x & 31][rl]);
+  const int kk = blockIdx.x * 32 + rl;
+  if ((threadIdx.x & 31) == 0 && kk < K) {
+    if (w32)
+      static_cast<float*>(dw)[kk] = s;
+    else
+      static_cast<__nv_bfloat16*>(dw)[kk] = __float2bfloat16_rn(s);
+  }
+}
+
+// Threads of a CTA that takes a row with two vectors a thread.
+int row_threads(int nvec, int v) { return ((nvec + v - 1) / v + 31) / 32 * 32; }
+
+// CTAs of the backward (also the rows of its workspace): two full SMs' worth
+// of threads each, no more than there are rows.
+int bwd_ctas(int64_t M, int nvec, int num_sms) {
+  if (nvec <= 128) {
+    const int64_t need = (M + WARP_ROWS - 1) / WARP_ROWS;
+    return static_cast<int>(need < 4 * num_sms ? need : 4 * num_sms);
+  }
+  const int per = 1024 / row_threads(nvec, 2) > 0 ? 1024 / row_threads(nvec, 2) : 1;
+  const int64_t most = static_cast<int64_t>(per) * num_sms;
+  return static_cast<int>(M < most ? M : most);
+}
+
+}  // namespace rms
+}  // namespace gl
+
+static int launched(const char** why) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return 0;
+  *why = cudaGetErrorString(e);
+  return -2;
+}
+
+// Launchers: 0 on a launch, -1 on a bad argument (why set), -2 on a launch error.
+int gl_launch_rms_norm_fwd(const void* x, const void* residual, const void* weight, int w32, float eps,
+                           int64_t M, int64_t K, void* h, void* y, void* q, float* s, float* rstd,
+                           cudaStream_t st, const char** why) {
+  using namespace gl::rms;
+  FwdArgs a{static_cast<const uint4*>(x), static_cast<const uint4*>(residual), weight,
+            static_cast<uint4*>(h), static_cast<uint4*>(y), static_cast<uint2*>(q), s, rstd, M,
+            static_cast<int>(K / 8), w32, 1.0f / static_cast<float>(K), eps};
+  const int n = a.nvec;
+  if (n <= 128) {
+    const unsigned ctas = static_cast<unsigned>((M + WARP_ROWS - 1) / WARP_ROWS);
+    const int t = 32 * WARP_ROWS;
+    if (n <= 32)
+      rms_norm_fwd_kernel<1, true><<<ctas, t, 0, st>>>(a);
+    else if (n <= 64)
+      rms_norm_fwd_kernel<2, true><<<ctas, t, 0, st>>>(a);
+    else
+      rms_norm_fwd_kernel<4, true><<<ctas, t, 0, st>>>(a);
+  } else {
+    rms_norm_fwd_kernel<2, false><<<static_cast<unsigned>(M), row_threads(n, 2), 0, st>>>(a);
+  }
+  return launched(why);
+}
+
+size_t gl_rms_norm_bwd_ws_bytes(int64_t M, int64_t K, int num_sms) {
+  return static_cast<size_t>(gl::rms::bwd_ctas(M, static_cast<int>(K / 8), num_sms)) * K * sizeof(float);
+}
+
+int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int w32,
+                           const float* rstd, int64_t M, int64_t K, void* dx, void* dw, void* ws,
+                           cudaStream_t st, int num_sms, const char** why) {
+  using namespace gl::rms;
+  BwdArgs a{static_cast<const uint4*>(dy), static_cast<const uint4*>(dh), static_cast<const uint4*>(h),
+            weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, static_cast<int>(K / 8),
+            w32, 1.0f / static_cast<float>(K)};
+  const int n = a.nvec, ctas = bwd_ctas(M, n, num_sms);
+  if (ctas > 0) {  // no rows: dw is a sum over nothing
+    if (n <= 32)
+      rms_norm_bwd_kernel<1, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+    else if (n <= 64)
+      rms_norm_bwd_kernel<2, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+    else if (n <= 128)
+      rms_norm_bwd_kernel<4, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+    else
+      rms_norm_bwd_kernel<2, false><<<ctas, row_threads(n, 2), 0, st>>>(a);
+    if (const int rc = launched(why)) return rc;
+  }
+  rms_norm_dw_kernel<<<static_cast<unsigned>((K + 31) / 32), 1024, 0, st>>>(
+      static_cast<const float*>(ws), ctas, static_cast<int>(K), w32, dw);
+  return launched(why);
+}

@@ -6,7 +6,8 @@ Op names and argument meaning mirror the Glaucis kernel templates
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+import contextlib
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -616,6 +617,155 @@ def chunk_gla(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g_gamma: Option
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, h0)):
         return _ChunkGLA.apply(q, k, v, g_gamma, g, h0, scale, chunk_size, exact_intra)
     return chunk_gla_fwd(q, k, v, g_gamma, scale, chunk_size, g=g, h0=h0, exact_intra=exact_intra).o
+
+
+# ---------------------------------------------------------------------------
+# RMS norm with the residual's addition
+# ---------------------------------------------------------------------------
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
+    """Checks that every tensor is a contiguous one on `first`'s CUDA device;
+    returns a context in which that device is the current one."""
+    _need_cuda(first, *rest)
+    dev = first.device
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError(f"all tensors of a call must be on one device, got {dev} and {t.device}")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+class RMSNormForward(NamedTuple):
+    """Result of rms_norm_fwd.  y (bf16) and q, s (e4m3 and its 1x128 scales)
+    are None unless asked for; h is the stored sum (x itself without a
+    residual); rstd (fp32 [M]) is the residual of the backward."""
+    y: Optional[torch.Tensor]
+    h: torch.Tensor
+    q: Optional[torch.Tensor]
+    s: Optional[torch.Tensor]
+    rstd: Optional[torch.Tensor]
+
+
+def _rms_check(x, weight, residual):
+    if x.dtype != torch.bfloat16 or x.dim() != 2:
+        raise ValueError("x must be a 2-D bf16 tensor")
+    M, K = x.shape
+    if weight.dtype not in (torch.bfloat16, torch.float32) or tuple(weight.shape) != (K,):
+        raise ValueError("weight must be bf16 or fp32 [K]")
+    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape):
+        raise ValueError("residual must be bf16 of x's shape")
+    return M, K
+
+
+def _rms_norm(x, weight, eps, residual, h, y, q, s, rstd):
+    """The launch itself: y, q and s, rstd are written where given."""
+    M, K = x.shape
+    _lib.check(_lib.load().gl_rms_norm_fwd(
+        x.data_ptr(), _ptr(residual), weight.data_ptr(), weight.dtype == torch.float32, eps, M, K,
+        h.data_ptr() if residual is not None else None, _ptr(y), _ptr(q), _ptr(s), _ptr(rstd), None,
+        _stream()), "gl_rms_norm_fwd")
+
+
+def rms_norm_quant_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                         residual: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                         s: Optional[torch.Tensor] = None, h: Optional[torch.Tensor] = None
+                         ) -> Tuple[torch.Tensor, ...]:
+    """RMS norm of x (+ residual) straight into the operand of gmm_fp8_fwd: x,
+    residual bf16 [M, K], weight bf16 or fp32 [K] -> (e4m3 [M, K], fp32 scales
+    [M, K/128]), and with a residual also h = bf16(x + residual), the stream
+    that goes on.  K a multiple of 128, at most 16384.
+
+    The layout and scales are quant_act_1x128's; the norm enters them in 32
+    bits, so the pair is rounded once.  q, s and h may be given preallocated;
+    h may be `x` or `residual` itself.
+    """
+    with _same_device(x, weight, residual):
+        M, K = _rms_check(x, weight, residual)
+        if h is not None and residual is None:
+            raise ValueError("h goes with a residual")
+        q = _out(q, (M, K), FP8, x.device, "q")
+        s = _out(s, (M, K // TILE), torch.float32, x.device, "s")
+        if residual is not None:
+            h = _out(h, (M, K), torch.bfloat16, x.device, "h")
+        _rms_norm(x, weight, eps, residual, h, None, q, s, None)
+    return (q, s) if residual is None else (q, s, h)
+
+
+def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                 residual: Optional[torch.Tensor] = None, output_quant: bool = False,
+                 y: Optional[torch.Tensor] = None, h: Optional[torch.Tensor] = None) -> RMSNormForward:
+    """Training forward of the RMS norm: h = bf16(x + residual) (x without
+    one), y = h / sqrt(mean(h^2) + eps) * weight in bf16, and what rms_norm_bwd
+    needs.  output_quant=True also returns y's e4m3 pair (rms_norm_quant_1x128)
+    from the same pass.  K a multiple of 8 (128 with output_quant), at most
+    16384; y and h may be given preallocated."""
+    with _same_device(x, weight, residual):
+        M, K = _rms_check(x, weight, residual)
+        if h is not None and residual is None:
+            raise ValueError("h goes with a residual")
+        y = _out(y, (M, K), torch.bfloat16, x.device, "y")
+        h = _out(h, (M, K), torch.bfloat16, x.device, "h") if residual is not None else x
+        q = s = None
+        if output_quant:
+            q = torch.empty((M, K), dtype=FP8, device=x.device)
+            s = torch.empty((M, K // TILE), dtype=torch.float32, device=x.device)
+        rstd = torch.empty(M, dtype=torch.float32, device=x.device)
+        _rms_norm(x, weight, eps, residual, h, y, q, s, rstd)
+    return RMSNormForward(y, h, q, s, rstd)
+
+
+def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, *,
+                 dh: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) for the gradients dy of y and dh of h (bf16 [M, K]), from
+    the forward's h and rstd.  dx is the gradient of x and of the residual;
+    dweight has weight's type and is summed in fp32 in a fixed order."""
+    with _same_device(h, dy, weight, rstd, dh):
+        M, K = _rms_check(h, weight, dh)
+        if dy.dtype != torch.bfloat16 or dy.shape != h.shape:
+            raise ValueError("dy must be bf16 of h's shape")
+        if rstd.dtype != torch.float32 or tuple(rstd.shape) != (M,):
+            raise ValueError("rstd must be fp32 [M]")
+        lib = _lib.load()
+        dx = torch.empty_like(h)
+        dw = torch.empty_like(weight)
+        ws_bytes = lib.gl_rms_norm_bwd_workspace_bytes(M, K)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device) if ws_bytes else None
+        _lib.check(lib.gl_rms_norm_bwd(dy.data_ptr(), _ptr(dh), h.data_ptr(), weight.data_ptr(),
+                                       weight.dtype == torch.float32, rstd.data_ptr(), M, K,
+                                       dx.data_ptr(), dw.data_ptr(), _ptr(ws), ws_bytes, None,
+                                       _stream()), "gl_rms_norm_bwd")
+    return dx, dw
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, residual):
+        f = rms_norm_fwd(x, weight, eps, residual=residual)
+        ctx.save_for_backward(f.h, weight, f.rstd)
+        ctx.set_materialize_grads(False)
+        return f.y if residual is None else (f.y, f.h)
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dh is not None:
+            dh = dh.to(torch.bfloat16).contiguous()
+        if dy is None:  # only the sum was used
+            return dh, None, None, dh
+        dx, dw = rms_norm_bwd(dy.to(torch.bfloat16).contiguous(), h, weight, rstd, dh=dh)
+        has_res = ctx.needs_input_grad[3]
+        return dx, dw, None, dx if has_res else None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+             residual: Optional[torch.Tensor] = None):
+    """RMS norm in bf16, differentiable in x, weight and residual: y, or with a
+    residual (y, h), h = bf16(x + residual) being the stream that goes on."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        return _RMSNorm.apply(x, weight, eps, residual)
+    f = rms_norm_fwd(x, weight, eps, residual=residual)
+    return f.y if residual is None else (f.y, f.h)
 
 
 def device_status() -> int:

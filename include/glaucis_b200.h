@@ -313,6 +313,47 @@ int gl_tgmm_fp8(const void* lq, const float* ls, const void* dq, const float* ds
                 const int32_t* group_sizes, int64_t G, int64_t M, int64_t K, int64_t N,
                 void* out, int out_dtype, int* err_word, void* stream);
 
+/*
+ * RMS norm with the residual's addition.  No counterpart in the reference,
+ * whose templates start at the experts' products: it makes their activations.
+ *   h = bf16(x + residual) (h = x when residual is NULL),
+ *   r = 1 / sqrt(mean_k h^2 + eps),  y = h * r * weight
+ *   x, residual  bf16 [M, K] row-major; residual may be NULL
+ *   weight       [K] bf16, or fp32 with weight_f32 != 0
+ *   h            bf16 [M, K], required with a residual and NULL without; may be
+ *                x's or the residual's own buffer
+ *   y            bf16 [M, K] or NULL
+ *   q, s         e4m3fn [M, K] and fp32 [M, K/128], the layout and scales of
+ *                gl_quant_act_1x128 (s = absmax(block of y)/448, 1.0 for an
+ *                all-zero block), both or neither NULL, K % 128 == 0 with them;
+ *                y enters them in 32 bits (not rounded to bf16 first)
+ *   rstd         fp32 [M], r of every row (the backward's residual), or NULL
+ * K % 8 == 0, 8 <= K <= GL_RMS_NORM_MAX_K, M <= 2^31 - 1; x, residual, weight,
+ * h, y and q 16-byte aligned.  Sums are fp32.  err_word is accepted for
+ * symmetry and never written (no device-side waits).
+ */
+#define GL_RMS_NORM_MAX_K 16384
+int gl_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_f32, float eps,
+                    int64_t M, int64_t K, void* h, void* y, void* q, float* s, float* rstd,
+                    int* err_word, void* stream);
+
+/*
+ * Backward of gl_rms_norm_fwd for the gradients dy of y and dh of h (dh may be
+ * NULL):  u = weight * dy, xh = h * rstd,
+ *   dx = rstd * (u - xh * mean_k(u * xh)) + dh   bf16 [M, K], the gradient of x
+ *                                                and of the residual
+ *   dweight = sum over rows of dy * xh           of weight's type, summed in
+ *                                                fp32 in a fixed order
+ * h, rstd as the forward wrote them (h = x without a residual).  workspace:
+ * gl_rms_norm_bwd_workspace_bytes(M, K) bytes on the current device (0 for an
+ * unsupported shape or M == 0), 16-byte aligned, not used by another call in
+ * flight.  M == 0 gives dweight = 0.
+ */
+size_t gl_rms_norm_bwd_workspace_bytes(int64_t M, int64_t K);
+int gl_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int weight_f32,
+                    const float* rstd, int64_t M, int64_t K, void* dx, void* dweight, void* workspace,
+                    size_t workspace_bytes, int* err_word, void* stream);
+
 /* Largest M*K accepted by gl_gmm_fp8_act_fwd_noalloc (activation elements). */
 #define GL_NOALLOC_MAX_ACT_ELEMS (16u * 1024u * 1024u)
 
