@@ -21,7 +21,8 @@ GL_EDEVICE = -3
 GL_OUT_BF16 = 0
 GL_OUT_F32 = 1
 GL_GLA_BF16_INTRA = 1
-DEV_CODES = {0: "ok", 1: "device wait timed out", 2: "invalid group_sizes (negative or sum > M)"}
+DEV_CODES = {0: "ok", 1: "device wait timed out", 2: "invalid group_sizes (negative or sum > M)",
+             3: "row index out of range"}
 
 # (name, restype, argtypes) for every symbol the header declares.
 _P, _I64, _I, _F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -59,6 +60,14 @@ SIGNATURES = {
     "gl_rms_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
     "gl_rms_norm_bwd": (_I, [_P, _P, _P, _P, _I, _P, _I64, _I64, _P, _P, _P, ctypes.c_size_t, _P,
                              _P]),
+    "gl_moe_route_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gl_moe_route_fwd": (_I, [_P, _I, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P, _P, _P,
+                              ctypes.c_size_t, _P, _P]),
+    "gl_moe_route_bwd": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "gl_moe_dispatch": (_I, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "gl_moe_combine": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "gl_moe_combine_bwd": (_I, [_P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,
+                                _P]),
     "gl_device_status": (_I, [_P, _P, ctypes.POINTER(ctypes.c_int)]),
     "gl_last_error": (ctypes.c_char_p, []),
     "gl_version": (ctypes.c_char_p, []),

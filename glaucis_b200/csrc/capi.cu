@@ -67,6 +67,26 @@ size_t gl_rms_norm_bwd_ws_bytes(int64_t M, int64_t K, int num_sms);
 int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int w32,
                            const float* rstd, int64_t M, int64_t K, void* dx, void* dw, void* ws,
                            cudaStream_t st, int num_sms, const char** why);
+size_t gl_moe_route_ws_bytes(int64_t E);
+int gl_launch_moe_route_fwd(const void* logits, int f32, const void* mask, int64_t T, int64_t E, int64_t k,
+                            int renorm, int32_t* ids, float* weights, int32_t* counts, int32_t* pos,
+                            float* loss, float* routed, void* ws, cudaStream_t st, int num_sms,
+                            const char** why);
+int gl_launch_moe_route_bwd(const void* logits, int f32, const void* mask, const int32_t* ids,
+                            const float* weights, const int32_t* counts, const float* routed,
+                            const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t k,
+                            int renorm, void* dlogits, cudaStream_t st, int num_sms, const char** why);
+int gl_launch_moe_dispatch(const void* x, int64_t row_bytes, const float* s, int64_t scales,
+                           const int32_t* pos, const int32_t* group_sizes, int64_t G, int64_t T, int64_t k,
+                           int64_t rows, void* out, float* out_s, int* err, cudaStream_t st, int num_sms,
+                           const char** why);
+int gl_launch_moe_combine(const void* y, int y_f32, const int32_t* pos, const float* weights,
+                          const void* residual, int64_t T, int64_t k, int64_t K, int64_t rows, void* out,
+                          int* err, cudaStream_t st, int num_sms, const char** why);
+int gl_launch_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t* pos,
+                              const float* weights, const int32_t* group_sizes, int64_t G, int64_t T,
+                              int64_t k, int64_t K, int64_t rows, void* dy, float* dweights, int* err,
+                              cudaStream_t st, int num_sms, const char** why);
 
 namespace {
 
@@ -693,6 +713,146 @@ int gl_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w
   const int rc = gl_launch_rms_norm_bwd(dy, dh, h, weight, weight_f32 != 0, rstd, M, K, dx, dweight,
                                         workspace, static_cast<cudaStream_t>(stream), d->num_sms, &why);
   if (rc != 0) return fail(rc == -1 ? GL_EINVAL : GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Router and exchange
+// ---------------------------------------------------------------------------
+static bool route_shape_ok(int64_t T, int64_t E) { return T >= 0 && T <= 0x7fffffff && E >= 1 && E <= 1024; }
+
+static int route_check(const char* f, int64_t T, int64_t E, int64_t topk) {
+  if (!route_shape_ok(T, E))
+    return fail(GL_EINVAL, std::string(f) + ": need 0 <= T < 2^31 and 1 <= E <= 1024");
+  if (topk < 1 || topk > E || topk > GL_MOE_MAX_TOPK)
+    return fail(GL_EINVAL, std::string(f) + ": need 1 <= topk <= min(E, 32)");
+  if (T * topk > 0x7fffffff) return fail(GL_EINVAL, std::string(f) + ": T * topk must fit in 31 bits");
+  return GL_OK;
+}
+
+size_t gl_moe_route_workspace_bytes(int64_t T, int64_t E) {
+  return route_shape_ok(T, E) ? gl_moe_route_ws_bytes(E) : 0;
+}
+
+int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64_t T, int64_t E,
+                     int64_t topk, int renormalize, int32_t* ids, float* weights, int32_t* counts,
+                     int32_t* pos, float* loss, float* routed, void* workspace, size_t workspace_bytes,
+                     int* err_word, void* stream) {
+  (void)err_word;
+  const char* f = "gl_moe_route_fwd";
+  if (int rc = route_check(f, T, E, topk)) return rc;
+  if (!counts || !loss || !routed || (T != 0 && (!logits || !ids || !weights || !pos)))
+    return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (!workspace || workspace_bytes < gl_moe_route_ws_bytes(E))
+    return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
+                                            "gl_moe_route_workspace_bytes gives");
+  if ((reinterpret_cast<uintptr_t>(workspace) & 3u) != 0)
+    return fail(GL_EINVAL, std::string(f) + ": the workspace must be 4-byte aligned");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_moe_route_fwd(logits, logits_f32 != 0, mask, T, E, topk, renormalize != 0, ids,
+                                         weights, counts, pos, loss, routed, workspace,
+                                         static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+int gl_moe_route_bwd(const void* logits, int logits_f32, const void* mask, const int32_t* ids,
+                     const float* weights, const int32_t* counts, const float* routed,
+                     const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t topk,
+                     int renormalize, void* dlogits, int* err_word, void* stream) {
+  (void)err_word;
+  const char* f = "gl_moe_route_bwd";
+  if (int rc = route_check(f, T, E, topk)) return rc;
+  if (T == 0) return GL_OK;
+  if (!logits || !ids || !weights || !counts || !routed || !dlogits)
+    return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_moe_route_bwd(logits, logits_f32 != 0, mask, ids, weights, counts, routed,
+                                         dweights, dloss, T, E, topk, renormalize != 0, dlogits,
+                                         static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+static int exchange_check(const char* f, int64_t T, int64_t topk, int64_t rows) {
+  if (T < 0 || topk < 1 || topk > GL_MOE_MAX_TOPK || T > 0x7fffffff || T * topk > 0x7fffffff)
+    return fail(GL_EINVAL, std::string(f) + ": need T >= 0, 1 <= topk <= 32 and T * topk < 2^31");
+  if (rows < 0 || rows > 0x7fffffff) return fail(GL_EINVAL, std::string(f) + ": need 0 <= rows < 2^31");
+  return GL_OK;
+}
+
+int gl_moe_dispatch(const void* x, int64_t row_bytes, const float* s, int64_t scales, const int32_t* pos,
+                    const int32_t* group_sizes, int64_t G, int64_t T, int64_t topk, int64_t rows, void* out,
+                    float* out_s, int* err_word, void* stream) {
+  const char* f = "gl_moe_dispatch";
+  if (int rc = exchange_check(f, T, topk, rows)) return rc;
+  if (row_bytes <= 0 || row_bytes % 16 != 0 || row_bytes > (int64_t(1) << 30))
+    return fail(GL_EINVAL, std::string(f) + ": row_bytes must be a positive multiple of 16");
+  if (scales < 0 || scales > (int64_t(1) << 30) || (s != nullptr && scales == 0))
+    return fail(GL_EINVAL, std::string(f) + ": bad number of scales");
+  if (G < 1 || G > 1024) return fail(GL_EINVAL, std::string(f) + ": need 1 <= G <= 1024");
+  if (!group_sizes || (T != 0 && (!x || !pos)) || (rows != 0 && !out))
+    return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (scales > 0 && ((T != 0 && !s) || (rows != 0 && !out_s)))
+    return fail(GL_EINVAL, std::string(f) + ": s and out_s go together");
+  if (!aligned16(x) || !aligned16(out))
+    return fail(GL_EINVAL, std::string(f) + ": x and out must be 16-byte aligned");
+  if (rows == 0 && T == 0) return GL_OK;
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_moe_dispatch(x, row_bytes, s, scales, pos, group_sizes, G, T, topk, rows, out,
+                                        out_s, err_word ? err_word : d->err,
+                                        static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+int gl_moe_combine(const void* y, int y_f32, const int32_t* pos, const float* weights, const void* residual,
+                   int64_t T, int64_t topk, int64_t K, int64_t rows, void* out, int* err_word,
+                   void* stream) {
+  const char* f = "gl_moe_combine";
+  if (int rc = exchange_check(f, T, topk, rows)) return rc;
+  if (K <= 0 || K % 8 != 0 || K > 16384)
+    return fail(GL_EINVAL, std::string(f) + ": K must be a multiple of 8 in 8..16384");
+  if (T == 0) return GL_OK;
+  if (!pos || !out || (rows != 0 && !y)) return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (!aligned16(y) || !aligned16(residual) || !aligned16(out))
+    return fail(GL_EINVAL, std::string(f) + ": y, residual and out must be 16-byte aligned");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_moe_combine(y, y_f32 != 0, pos, weights, residual, T, topk, K, rows, out,
+                                       err_word ? err_word : d->err, static_cast<cudaStream_t>(stream),
+                                       d->num_sms, &why);
+  if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+int gl_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t* pos, const float* weights,
+                       const int32_t* group_sizes, int64_t G, int64_t T, int64_t topk, int64_t K,
+                       int64_t rows, void* dy, float* dweights, int* err_word, void* stream) {
+  const char* f = "gl_moe_combine_bwd";
+  if (int rc = exchange_check(f, T, topk, rows)) return rc;
+  if (K <= 0 || K % 8 != 0 || K > 16384)
+    return fail(GL_EINVAL, std::string(f) + ": K must be a multiple of 8 in 8..16384");
+  if (G < 1 || G > 1024) return fail(GL_EINVAL, std::string(f) + ": need 1 <= G <= 1024");
+  if (!group_sizes || (T != 0 && (!dout || !pos || !weights || !dweights)) || (rows != 0 && (!y || !dy)))
+    return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (!aligned16(dout) || !aligned16(y) || !aligned16(dy))
+    return fail(GL_EINVAL, std::string(f) + ": dout, y and dy must be 16-byte aligned");
+  if (rows == 0 && T == 0) return GL_OK;
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_moe_combine_bwd(dout, y, y_f32 != 0, pos, weights, group_sizes, G, T, topk, K,
+                                           rows, dy, dweights, err_word ? err_word : d->err,
+                                           static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
   return GL_OK;
 }
 

@@ -1,0 +1,504 @@
+// Router of a mixture of experts: softmax over E experts, the k largest logits
+// of every token (ties to the lowest expert), the tokens each expert gets
+// (group_sizes of the grouped matmul), the row of every choice when the
+// choices are sorted by (expert, token, slot), and the balance loss
+//   loss = E * sum_e f_e P_e,  f_e = counts_e / sum(counts),
+//   P_e = mean of the softmax over the routed tokens;
+// and the gradient of the logits for gradients of the weights and the loss.
+//
+// A warp takes a token, lane l holding experts l, l + 32, ...: the softmax's
+// sums and the k rounds of the selection are warp reductions on registers.  A
+// round finds the largest key with one redux.max and its lowest expert with
+// one redux.min, so it is bound by the latency of these (E floats a token are
+// little to read).  Rows need the counts of all earlier tokens: each CTA takes
+// consecutive tokens and leaves its counts per expert, a second launch (not
+// needed when one CTA takes all tokens) adds up those of the CTAs before it
+// and ranks its choices in order.  Counts are integers and the loss's sums run
+// in a fixed order over warps and CTAs: results do not depend on timing.
+#include "common.cuh"
+
+namespace gl {
+namespace route {
+
+constexpr uint32_t FULL = 0xFFFFFFFFu;
+constexpr int MAX_CTAS = 148;
+
+// Warps of a CTA: the per-warp rows of E values must fit 32 KB.
+template <int V>
+constexpr int warps() {
+  return V <= 8 ? 32 : V == 16 ? 16 : 8;
+}
+
+struct Args {
+  const void* logits;
+  const uint8_t* mask;  // or null
+  int64_t T;
+  int E, k, f32, renorm;
+  int64_t chunk;        // tokens of a CTA
+  int* ids;
+  float* weights;
+  int* counts;
+  int* pos;
+  float* loss;
+  float* routed;        // routed tokens, as a float
+  int* hist;            // [CTAs, E]
+  float* psum;          // [CTAs, E]
+  int* live;            // [CTAs]
+};
+
+template <int V>
+struct Shared {
+  union {
+    float psum[warps<V>()][32 * V];     // each warp's sum of the softmax
+    uint16_t cnt[warps<V>()][32 * V];   // choices of an expert in a batch of entries
+  };
+  int hist[32 * V];   // this CTA's counts, then the row of an expert's next choice
+  int total[32 * V];
+  float red[32];
+  int live;
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+
+__device__ __forceinline__ float load_logit(const void* p, int f32, int64_t i) {
+  return f32 ? __ldg(static_cast<const float*>(p) + i)
+             : __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
+}
+
+// Orders floats as unsigned integers (+0 and -0 alike); -inf and NaN, which
+// are never chosen, give 0.
+__device__ __forceinline__ uint32_t key_of(float z) {
+  if (!(z > -INFINITY)) return 0;
+  const uint32_t b = __float_as_uint(z + 0.0f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+}
+
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// Softmax numerators of a token's logits z (lane l: experts l + 32 i); returns
+// 1 / their sum.
+template <int V>
+__device__ __forceinline__ float softmax(const float (&z)[V], float (&e)[V], float& zmax) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = fmaxf(m, z[i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+  zmax = m;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    e[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - m);
+    s += e[i];
+  }
+  return 1.0f / warp_sum(s);
+}
+
+// A token takes part when the mask keeps it and a logit of it is not -inf.
+template <int V>
+__device__ __forceinline__ bool load_token(const Args& a, int64_t t, float (&z)[V]) {
+  const int lane = threadIdx.x & 31;
+  const bool kept = a.mask == nullptr || __ldg(a.mask + t) != 0;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    z[i] = e < a.E && kept ? load_logit(a.logits, a.f32, t * a.E + e) : -INFINITY;
+    any = any || z[i] != -INFINITY;
+  }
+  return __any_sync(FULL, any);
+}
+
+// Routes tokens [t0, t1): ids, weights; counts into sh.hist, softmax sums and
+// the number of routed tokens into the CTA's slots.
+template <int V>
+__device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& sh, int cta) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) sh.hist[e] = 0;
+  if (threadIdx.x == 0) sh.live = 0;
+  __syncthreads();
+  float psum[V] = {};
+  int live = 0;
+  for (int64_t t = t0 + warp; t < t1; t += warps<V>()) {
+    float z[V], e[V], zmax;
+    const bool in = load_token<V>(a, t, z);
+    int id = -1;
+    float p = 0.0f;
+    if (in) {
+      ++live;
+      const float inv = softmax<V>(z, e, zmax);
+      uint32_t key[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        psum[i] += e[i] * inv;
+        key[i] = key_of(z[i]);
+      }
+      for (int j = 0; j < a.k; ++j) {
+        uint32_t m = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) m = max(m, key[i]);
+        m = __reduce_max_sync(FULL, m);
+        if (m == 0) break;  // nothing left to choose
+        uint32_t at = FULL;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i)
+          if (key[i] == m) at = static_cast<uint32_t>(lane + 32 * i);
+        at = __reduce_min_sync(FULL, at);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (at == static_cast<uint32_t>(lane + 32 * i)) key[i] = 0;
+        if (lane == j) {
+          id = static_cast<int>(at);
+          p = expf(of_key(m) - zmax) * inv;
+        }
+      }
+      if (a.renorm) {
+        const float s = warp_sum(p);
+        if (id >= 0) p /= s;
+      }
+    }
+    if (lane < a.k) {
+      a.ids[t * a.k + lane] = id;
+      a.weights[t * a.k + lane] = p;
+      if (id >= 0) atomicAdd(&sh.hist[id], 1);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sh.psum[warp][lane + 32 * i] = psum[i];
+  if (lane == 0 && live) atomicAdd(&sh.live, live);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int w = 0; w < warps<V>(); ++w) s += sh.psum[w][e];
+    a.psum[static_cast<int64_t>(cta) * a.E + e] = s;
+    a.hist[static_cast<int64_t>(cta) * a.E + e] = sh.hist[e];
+  }
+  if (threadIdx.x == 0) a.live[cta] = sh.live;
+}
+
+// sh.total: choices of every expert; sh.hist: the first row of this CTA's
+// choices of it.  `ctas` CTAs' counts, `cta` of them before this one.
+template <int V>
+__device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
+  for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) sh.total[e] = sh.hist[e] = 0;
+  __syncthreads();
+  const int slices = blockDim.x >= 32 * V ? blockDim.x / (32 * V) : 1;
+  for (int i = threadIdx.x; i < slices * 32 * V; i += blockDim.x) {
+    const int e = i % (32 * V);
+    if (e >= a.E) continue;
+    int before = 0, total = 0;
+    for (int b = i / (32 * V); b < ctas; b += slices) {
+      const int h = a.hist[static_cast<int64_t>(b) * a.E + e];
+      total += h;
+      before += b < cta ? h : 0;
+    }
+    if (total) atomicAdd(&sh.total[e], total);
+    if (before) atomicAdd(&sh.hist[e], before);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    // exclusive scan over the experts, V consecutive ones a lane
+    const int lane = threadIdx.x;
+    int own = 0;
+#pragma unroll 4
+    for (int i = 0; i < V; ++i) own += sh.total[lane * V + i];
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(FULL, inc, o);
+      if (lane >= o) inc += v;
+    }
+    int run = inc - own;
+#pragma unroll 4
+    for (int i = 0; i < V; ++i) {
+      sh.hist[lane * V + i] += run;
+      run += sh.total[lane * V + i];
+    }
+  }
+  __syncthreads();
+}
+
+// Rows of the choices of tokens [t0, t1), a batch of one choice a thread at a
+// time: rank among the batch's earlier choices of the same expert (within the
+// warp by match, over the warps by a column of counts).
+template <int V>
+__device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n0 = t0 * a.k, n1 = t1 * a.k;
+  for (int64_t b = n0; b < n1; b += blockDim.x) {
+    uint32_t* zero = reinterpret_cast<uint32_t*>(&sh.cnt[0][0]);
+    for (int i = threadIdx.x; i < warps<V>() * 16 * V; i += blockDim.x) zero[i] = 0;
+    __syncthreads();
+    const int64_t n = b + threadIdx.x;
+    const int id = n < n1 ? a.ids[n] : -1;
+    const uint32_t same = __match_any_sync(FULL, id);
+    const int rank = __popc(same & ((1u << lane) - 1u));
+    if (id >= 0 && rank == 0) sh.cnt[warp][id] = static_cast<uint16_t>(__popc(same));
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+      int run = 0;
+#pragma unroll 8
+      for (int w = 0; w < warps<V>(); ++w) {
+        const int c = sh.cnt[w][e];
+        sh.cnt[w][e] = static_cast<uint16_t>(run);
+        run += c;
+      }
+      sh.total[e] = run;
+    }
+    __syncthreads();
+    if (n < n1) a.pos[n] = id >= 0 ? sh.hist[id] + sh.cnt[warp][id] + rank : -1;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) sh.hist[e] += sh.total[e];
+  }
+}
+
+// counts, the loss and the number of routed tokens (sh.total: all choices).
+template <int V>
+__device__ void finish(const Args& a, Shared<V>& sh, int ctas) {
+  float part = 0.0f, chosen = 0.0f;
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    float p = 0.0f;
+    for (int b = 0; b < ctas; ++b) p += a.psum[static_cast<int64_t>(b) * a.E + e];
+    a.counts[e] = sh.total[e];
+    part = fmaf(static_cast<float>(sh.total[e]), p, part);
+    chosen += static_cast<float>(sh.total[e]);
+  }
+  int n = 0;
+  for (int b = threadIdx.x & 31; b < ctas; b += 32) n += a.live[b];
+  n = __reduce_add_sync(FULL, n);
+  part = warp_sum(part);
+  chosen = warp_sum(chosen);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+  if (lane == 0) sh.red[warp] = part;
+  __syncthreads();
+  part = warp_sum(lane < warps<V>() ? sh.red[lane] : 0.0f);
+  __syncthreads();
+  if (lane == 0) sh.red[warp] = chosen;
+  __syncthreads();
+  chosen = warp_sum(lane < warps<V>() ? sh.red[lane] : 0.0f);
+  if (threadIdx.x == 0) {
+    const float tokens = static_cast<float>(max(n, 1));
+    *a.loss = static_cast<float>(a.E) * (part / fmaxf(chosen, 1.0f) / tokens);
+    *a.routed = tokens;
+  }
+}
+
+// kOne: a single CTA takes every token and finishes; else the first of two
+// launches.
+template <int V, bool kOne>
+__global__ void __launch_bounds__(32 * warps<V>()) route_kernel(const Args a) {
+  __shared__ Shared<V> sh;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
+  const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
+  route_tokens<V>(a, t0, t1, sh, blockIdx.x);
+  if (kOne) {
+    __syncthreads();
+    first_rows<V>(a, sh, 1, 0);
+    finish<V>(a, sh, 1);
+    __syncthreads();
+    assign_rows<V>(a, sh, t0, t1);
+  }
+}
+
+// Second launch: the CTAs of the first rank their choices, one more finishes.
+template <int V>
+__global__ void __launch_bounds__(32 * warps<V>()) rank_kernel(const Args a) {
+  __shared__ Shared<V> sh;
+  cudaGridDependencySynchronize();
+  const int ctas = gridDim.x - 1, cta = blockIdx.x;
+  first_rows<V>(a, sh, ctas, cta);
+  if (cta == ctas) {
+    finish<V>(a, sh, ctas);
+    return;
+  }
+  const int64_t t0 = static_cast<int64_t>(cta) * a.chunk;
+  const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
+  assign_rows<V>(a, sh, t0, t1);
+}
+
+struct BwdArgs {
+  const int* ids;
+  const float* weights;
+  const int* counts;
+  const float* routed;
+  const float* dweights;  // or null
+  const float* dloss;     // or null
+  void* dlogits;
+};
+
+__device__ __forceinline__ void store_logit(void* p, int f32, int64_t i, float v) {
+  if (f32)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// dlogit_e = p_e (c_e + sel_e - sum_e' p_e' (c_e' + sel_e')), c_e = dloss E f_e / n
+// for the loss and sel_e the weights' part on the chosen experts.
+template <int V>
+__global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdArgs b) {
+  const int lane = threadIdx.x & 31;
+  float c[V], chosen = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = lane + 32 * i;
+    c[i] = e < a.E ? static_cast<float>(__ldg(b.counts + e)) : 0.0f;
+    chosen += c[i];
+  }
+  chosen = fmaxf(warp_sum(chosen), 1.0f);
+  const float scale = b.dloss ? __ldg(b.dloss) * static_cast<float>(a.E) / __ldg(b.routed) / chosen : 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] *= scale;
+  const int64_t warps_all = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.T;
+       t += warps_all) {
+    float z[V], e[V], zmax;
+    const bool in = load_token<V>(a, t, z);
+    if (!in) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (lane + 32 * i < a.E) store_logit(b.dlogits, a.f32, t * a.E + lane + 32 * i, 0.0f);
+      continue;
+    }
+    int id = -1;
+    float sel = 0.0f, w = 0.0f;
+    if (lane < a.k) {
+      id = __ldg(b.ids + t * a.k + lane);
+      if (id < 0 || id >= a.E) id = -1;
+      w = __ldg(b.weights + t * a.k + lane);
+      sel = b.dweights && id >= 0 ? __ldg(b.dweights + t * a.k + lane) : 0.0f;
+    }
+    const float inv = softmax<V>(z, e, zmax);
+    const float p_sel = id >= 0 ? expf(load_logit(a.logits, a.f32, t * a.E + id) - zmax) * inv : 0.0f;
+    if (a.renorm) {
+      const float dot = warp_sum(id >= 0 ? sel * w : 0.0f);
+      const float s = warp_sum(p_sel);
+      sel = id >= 0 ? (sel - dot) / s : 0.0f;
+    }
+    float dot = p_sel * sel;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      e[i] *= inv;
+      dot = fmaf(e[i], c[i], dot);
+    }
+    dot = warp_sum(dot);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane + 32 * i < a.E)
+        store_logit(b.dlogits, a.f32, t * a.E + lane + 32 * i, e[i] * (c[i] - dot));
+    __syncwarp();
+    // the chosen experts' values over those just written (other lanes' stores,
+    // ordered by the warp's barrier)
+    if (id >= 0)
+      store_logit(b.dlogits, a.f32, t * a.E + id,
+                  p_sel * (static_cast<float>(__ldg(b.counts + id)) * scale + sel - dot));
+  }
+}
+
+// CTAs of the forward: one when its warps take every token in a few rounds
+// (a second launch costs more than those rounds), else one per SM at most.
+int fwd_ctas(int64_t T, int w, int num_sms) {
+  if (T <= 2 * w) return 1;
+  const int64_t need = (T + w - 1) / w;
+  const int most = num_sms < MAX_CTAS ? num_sms : MAX_CTAS;
+  return static_cast<int>(need < most ? need : most);
+}
+
+template <int V>
+int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
+  Args a = a0;
+  const int ctas = fwd_ctas(a.T, warps<V>(), num_sms);
+  a.chunk = a.T > 0 ? (a.T + ctas - 1) / ctas : 1;
+  cudaError_t e;
+  if (ctas == 1) {
+    route_kernel<V, true><<<1, 32 * warps<V>(), 0, st>>>(a);
+    e = cudaGetLastError();
+  } else {
+    route_kernel<V, false><<<ctas, 32 * warps<V>(), 0, st>>>(a);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) {
+      // launched while the first runs out; it waits for it on the device
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(ctas + 1);
+      cfg.blockDim = dim3(32 * warps<V>());
+      cfg.stream = st;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, rank_kernel<V>, a);
+    }
+  }
+  if (e == cudaSuccess) return 0;
+  *why = cudaGetErrorString(e);
+  return -2;
+}
+
+template <int V>
+int bwd(const Args& a, const BwdArgs& b, int num_sms, cudaStream_t st, const char** why) {
+  const int64_t need = (a.T + 7) / 8;
+  const int64_t most = static_cast<int64_t>(num_sms) * (V <= 8 ? 8 : 4);
+  route_bwd_kernel<V><<<static_cast<unsigned>(need < most ? need : most), 256, 0, st>>>(a, b);
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return 0;
+  *why = cudaGetErrorString(e);
+  return -2;
+}
+
+}  // namespace route
+}  // namespace gl
+
+// hist and psum of every CTA, then its number of routed tokens.
+size_t gl_moe_route_ws_bytes(int64_t E) {
+  return static_cast<size_t>(gl::route::MAX_CTAS) * (2 * static_cast<size_t>(E) + 1) * 4;
+}
+
+// Launchers: 0 on a launch, -2 on a launch error (why set).
+int gl_launch_moe_route_fwd(const void* logits, int f32, const void* mask, int64_t T, int64_t E, int64_t k,
+                            int renorm, int32_t* ids, float* weights, int32_t* counts, int32_t* pos,
+                            float* loss, float* routed, void* ws, cudaStream_t st, int num_sms,
+                            const char** why) {
+  using namespace gl::route;
+  int* hist = static_cast<int*>(ws);
+  float* psum = reinterpret_cast<float*>(hist + MAX_CTAS * E);
+  int* live = reinterpret_cast<int*>(psum + MAX_CTAS * E);
+  const Args a{logits, static_cast<const uint8_t*>(mask), T, static_cast<int>(E), static_cast<int>(k), f32,
+               renorm, 0, ids, weights, counts, pos, loss, routed, hist, psum, live};
+  if (E <= 32) return fwd<1>(a, num_sms, st, why);
+  if (E <= 64) return fwd<2>(a, num_sms, st, why);
+  if (E <= 128) return fwd<4>(a, num_sms, st, why);
+  if (E <= 256) return fwd<8>(a, num_sms, st, why);
+  if (E <= 512) return fwd<16>(a, num_sms, st, why);
+  return fwd<32>(a, num_sms, st, why);
+}
+
+int gl_launch_moe_route_bwd(const void* logits, int f32, const void* mask, const int32_t* ids,
+                            const float* weights, const int32_t* counts, const float* routed,
+                            const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t k,
+                            int renorm, void* dlogits, cudaStream_t st, int num_sms, const char** why) {
+  using namespace gl::route;
+  Args a = {};
+  a.logits = logits;
+  a.mask = static_cast<const uint8_t*>(mask);
+  a.T = T;
+  a.E = static_cast<int>(E);
+  a.k = static_cast<int>(k);
+  a.f32 = f32;
+  a.renorm = renorm;
+  const BwdArgs b{ids, weights, counts, routed, dweights, dloss, dlogits};
+  if (E <= 32) return bwd<1>(a, b, num_sms, st, why);
+  if (E <= 64) return bwd<2>(a, b, num_sms, st, why);
+  if (E <= 128) return bwd<4>(a, b, num_sms, st, why);
+  if (E <= 256) return bwd<8>(a, b, num_sms, st, why);
+  if (E <= 512) return bwd<16>(a, b, num_sms, st, why);
+  return bwd<32>(a, b, num_sms, st, why);
+}

@@ -768,6 +768,286 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     return f.y if residual is None else (f.y, f.h)
 
 
+# ---------------------------------------------------------------------------
+# Router: top-k, group sizes, rows in expert order, balance loss
+# ---------------------------------------------------------------------------
+class MoERouting(NamedTuple):
+    """Result of moe_route.  ids (int32 [T, topk]) are the chosen experts in
+    falling order of their logits, weights (fp32) their softmax, counts (int32
+    [E]) the group_sizes of the grouped matmul, pos (int32 [T, topk]) the row
+    of every choice in expert order; slots without an expert have ids and pos
+    -1 and weight 0.  routed, mask and renormalize are kept for the backward."""
+    ids: torch.Tensor
+    weights: torch.Tensor
+    counts: torch.Tensor
+    pos: torch.Tensor
+    balance_loss: torch.Tensor
+    routed: torch.Tensor
+    mask: Optional[torch.Tensor]
+    renormalize: bool
+
+
+def _route_check(logits, mask):
+    if logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2:
+        raise ValueError("logits must be a 2-D bf16 or fp32 tensor")
+    T, E = logits.shape
+    if mask is not None and (mask.dtype != torch.bool or tuple(mask.shape) != (T,)):
+        raise ValueError("mask must be bool [T]")
+    return T, E
+
+
+def moe_route_fwd(logits: torch.Tensor, topk: int, *, mask: Optional[torch.Tensor] = None,
+                  renormalize: bool = True) -> MoERouting:
+    """Routes every token (logits [T, E], bf16 or fp32) to its topk experts:
+    softmax, the largest logits with ties to the lowest expert, their weights
+    (over their sum with renormalize), the experts' counts, the rows in expert
+    order, and the balance loss E * sum_e f_e P_e (f_e: share of the choices,
+    P_e: mean probability), which is 1 for an even split.
+
+    A logit of -inf takes its expert out for that token; tokens with mask
+    False, or with no logit above -inf, are not routed and are in no sum.  A
+    NaN is never chosen and makes its token's weights and the loss NaN.
+    E <= 1024, topk <= 32."""
+    with _same_device(logits, mask):
+        T, E = _route_check(logits, mask)
+        dev = logits.device
+        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+        pos = torch.empty((T, topk), dtype=torch.int32, device=dev)
+        weights = torch.empty((T, topk), dtype=torch.float32, device=dev)
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        routed = torch.empty((), dtype=torch.float32, device=dev)
+        lib = _lib.load()
+        ws_bytes = lib.gl_moe_route_workspace_bytes(T, E)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _lib.check(lib.gl_moe_route_fwd(logits.data_ptr(), logits.dtype == torch.float32, _ptr(mask), T, E,
+                                        topk, renormalize, ids.data_ptr(), weights.data_ptr(),
+                                        counts.data_ptr(), pos.data_ptr(), loss.data_ptr(),
+                                        routed.data_ptr(), ws.data_ptr(), ws_bytes, None, _stream()),
+                   "gl_moe_route_fwd")
+    return MoERouting(ids, weights, counts, pos, loss, routed, mask, renormalize)
+
+
+def moe_route_bwd(logits: torch.Tensor, routing: MoERouting, dweights: Optional[torch.Tensor],
+                  dloss: Optional[torch.Tensor]) -> torch.Tensor:
+    """dlogits (of logits' type) for the gradients of routing.weights (fp32
+    [T, topk]) and of the balance loss (fp32, one element; either may be None).
+    The choices and counts are constants of the differentiation."""
+    r = routing
+    with _same_device(logits, r.ids, r.weights, r.counts, r.routed, r.mask, dweights, dloss):
+        T, E = _route_check(logits, r.mask)
+        topk = r.ids.shape[1]
+        if tuple(r.ids.shape) != (T, topk) or r.weights.shape != r.ids.shape or r.counts.numel() != E:
+            raise ValueError("routing does not belong to these logits")
+        if dweights is not None and (dweights.dtype != torch.float32 or dweights.shape != r.ids.shape):
+            raise ValueError("dweights must be fp32 [T, topk]")
+        if dloss is not None and (dloss.dtype != torch.float32 or dloss.numel() != 1):
+            raise ValueError("dloss must be fp32 with one element")
+        dlogits = torch.empty_like(logits)
+        _lib.check(_lib.load().gl_moe_route_bwd(
+            logits.data_ptr(), logits.dtype == torch.float32, _ptr(r.mask), r.ids.data_ptr(),
+            r.weights.data_ptr(), r.counts.data_ptr(), r.routed.data_ptr(), _ptr(dweights), _ptr(dloss),
+            T, E, topk, r.renormalize, dlogits.data_ptr(), None, _stream()), "gl_moe_route_bwd")
+    return dlogits
+
+
+class _MoERoute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk, mask, renormalize):
+        r = moe_route_fwd(logits, topk, mask=mask, renormalize=renormalize)
+        ctx.save_for_backward(logits, r.ids, r.weights, r.counts, r.routed, mask)
+        ctx.renormalize = renormalize
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(r.ids, r.counts, r.pos, r.routed)
+        return r.ids, r.weights, r.counts, r.pos, r.balance_loss, r.routed
+
+    @staticmethod
+    def backward(ctx, _ids, dweights, _counts, _pos, dloss, _routed):
+        if dweights is None and dloss is None:
+            return None, None, None, None
+        logits, ids, weights, counts, routed, mask = ctx.saved_tensors
+        r = MoERouting(ids, weights, counts, None, None, routed, mask, ctx.renormalize)
+        dweights = dweights.float().contiguous() if dweights is not None else None
+        dloss = dloss.float().contiguous() if dloss is not None else None
+        return moe_route_bwd(logits, r, dweights, dloss), None, None, None
+
+
+def moe_route(logits: torch.Tensor, topk: int, *, mask: Optional[torch.Tensor] = None,
+              renormalize: bool = True) -> MoERouting:
+    """moe_route_fwd, its weights and balance loss differentiable in logits."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = _MoERoute.apply(logits, topk, mask, renormalize)
+        return MoERouting(*out, mask, renormalize)
+    return moe_route_fwd(logits, topk, mask=mask, renormalize=renormalize)
+
+
+# ---------------------------------------------------------------------------
+# Rows into expert order and back
+# ---------------------------------------------------------------------------
+def _pos_check(pos, group_sizes=None):
+    if pos.dtype != torch.int32 or pos.dim() != 2:
+        raise ValueError("pos must be int32 [T, topk]")
+    if group_sizes is not None and (group_sizes.dtype != torch.int32 or group_sizes.dim() != 1):
+        raise ValueError("group_sizes must be int32 [G]")
+    return pos.shape
+
+
+def _dispatch(x, s, pos, group_sizes, rows, out, out_s):
+    T, topk = pos.shape
+    scales = 0 if s is None else s.shape[1]
+    _lib.check(_lib.load().gl_moe_dispatch(x.data_ptr(), x.shape[1] * x.element_size(), _ptr(s), scales,
+                                           pos.data_ptr(), group_sizes.data_ptr(), group_sizes.numel(), T,
+                                           topk, rows, out.data_ptr(), _ptr(out_s), None, _stream()),
+               "gl_moe_dispatch")
+
+
+def moe_dispatch_fwd(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
+                     rows: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The forward of moe_dispatch, with `out` optionally preallocated."""
+    with _same_device(x, pos, group_sizes):
+        T, topk = _pos_check(pos, group_sizes)
+        if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or x.shape[0] != T:
+            raise ValueError("x must be bf16 or fp32 [T, K]")
+        rows = T * topk if rows is None else int(rows)
+        out = _out(out, (rows, x.shape[1]), x.dtype, x.device, "out")
+        _dispatch(x, None, pos, group_sizes, rows, out, None)
+    return out
+
+
+def moe_dispatch_quant(q: torch.Tensor, s: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
+                       rows: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                       out_s: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """moe_dispatch of quantised rows: q e4m3 [T, K] and s fp32 [T, K/128]
+    (quant_act_1x128 or rms_norm_quant_1x128 of the tokens) -> the operands of
+    gmm_fp8_fwd, quantised once per token instead of once per choice.  Rows
+    past sum(group_sizes) are zeros with scale 1."""
+    with _same_device(q, s, pos, group_sizes):
+        T, topk = _pos_check(pos, group_sizes)
+        if q.dtype != FP8 or q.dim() != 2 or q.shape[0] != T:
+            raise ValueError("q must be e4m3 [T, K]")
+        if s.dtype != torch.float32 or tuple(s.shape) != (T, q.shape[1] // TILE) or q.shape[1] % TILE:
+            raise ValueError("s must be fp32 [T, K/128], K a multiple of 128")
+        rows = T * topk if rows is None else int(rows)
+        out = _out(out, (rows, q.shape[1]), FP8, q.device, "out")
+        out_s = _out(out_s, (rows, s.shape[1]), torch.float32, q.device, "out_s")
+        _dispatch(q, s, pos, group_sizes, rows, out, out_s)
+    return out, out_s
+
+
+def _combine(y, pos, weights, residual, out):
+    T, topk = pos.shape
+    rows, K = y.shape
+    _lib.check(_lib.load().gl_moe_combine(y.data_ptr(), y.dtype == torch.float32, pos.data_ptr(),
+                                          _ptr(weights), _ptr(residual), T, topk, K, rows, out.data_ptr(),
+                                          None, _stream()), "gl_moe_combine")
+
+
+def moe_dispatch_bwd(dout: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+    """Gradient bf16 [T, K] of moe_dispatch's x for dout [rows, K] (bf16 or
+    fp32): the sum of a token's rows, in fp32."""
+    with _same_device(dout, pos):
+        T, _ = _pos_check(pos)
+        if dout.dtype not in (torch.bfloat16, torch.float32) or dout.dim() != 2:
+            raise ValueError("dout must be bf16 or fp32 [rows, K]")
+        dx = torch.empty((T, dout.shape[1]), dtype=torch.bfloat16, device=dout.device)
+        _combine(dout, pos, None, None, dx)
+    return dx
+
+
+class _MoEDispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, group_sizes, rows):
+        ctx.save_for_backward(pos)
+        return moe_dispatch_fwd(x, pos, group_sizes, rows)
+
+    @staticmethod
+    def backward(ctx, dout):
+        return moe_dispatch_bwd(dout.to(torch.bfloat16).contiguous(), ctx.saved_tensors[0]), None, None, None
+
+
+def moe_dispatch(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
+                 rows: Optional[int] = None) -> torch.Tensor:
+    """Rows of the tokens in expert order: out[pos[t, j]] = x[t] (bf16 [T, K])
+    for the pos and counts of moe_route; the lhs of gmm_fp8_blockwise with
+    group_sizes = counts.  `rows` (default T * topk) is the number of output
+    rows; those past sum(group_sizes) are zero.  Differentiable in x (bf16)."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        if x.dtype != torch.bfloat16:
+            raise ValueError("the differentiable moe_dispatch takes bf16")
+        return _MoEDispatch.apply(x, pos, group_sizes, rows)
+    return moe_dispatch_fwd(x, pos, group_sizes, rows)
+
+
+def _combine_check(y, pos, weights):
+    T, topk = _pos_check(pos)
+    if y.dtype not in (torch.bfloat16, torch.float32) or y.dim() != 2:
+        raise ValueError("y must be bf16 or fp32 [rows, K]")
+    if weights.dtype != torch.float32 or weights.shape != pos.shape:
+        raise ValueError("weights must be fp32 [T, topk]")
+    return T, topk
+
+
+def moe_combine_fwd(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, *,
+                    residual: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The forward of moe_combine, with `out` optionally preallocated (it may
+    be `residual` itself)."""
+    with _same_device(y, pos, weights, residual):
+        T, _ = _combine_check(y, pos, weights)
+        if residual is not None and (residual.dtype != torch.bfloat16
+                                     or tuple(residual.shape) != (T, y.shape[1])):
+            raise ValueError("residual must be bf16 [T, K]")
+        out = _out(out, (T, y.shape[1]), torch.bfloat16, y.device, "out")
+        _combine(y, pos, weights, residual, out)
+    return out
+
+
+def moe_combine_bwd(dout: torch.Tensor, y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor,
+                    group_sizes: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dy, dweights) of moe_combine for dout (bf16 [T, K]): dy has y's type,
+    its rows past sum(group_sizes) are zero; the residual's gradient is dout."""
+    with _same_device(y, dout, pos, weights, group_sizes):
+        T, topk = _combine_check(y, pos, weights)
+        _pos_check(pos, group_sizes)
+        rows, K = y.shape
+        if dout.dtype != torch.bfloat16 or tuple(dout.shape) != (T, K):
+            raise ValueError("dout must be bf16 [T, K]")
+        dy = torch.empty_like(y)
+        dw = torch.empty_like(weights)
+        _lib.check(_lib.load().gl_moe_combine_bwd(
+            dout.data_ptr(), y.data_ptr(), y.dtype == torch.float32, pos.data_ptr(), weights.data_ptr(),
+            group_sizes.data_ptr(), group_sizes.numel(), T, topk, K, rows, dy.data_ptr(), dw.data_ptr(),
+            None, _stream()), "gl_moe_combine_bwd")
+    return dy, dw
+
+
+class _MoECombine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, pos, weights, group_sizes, residual):
+        ctx.save_for_backward(y, pos, weights, group_sizes)
+        return moe_combine_fwd(y, pos, weights, residual=residual)
+
+    @staticmethod
+    def backward(ctx, dout):
+        y, pos, weights, group_sizes = ctx.saved_tensors
+        dout = dout.to(torch.bfloat16).contiguous()
+        dy = dw = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[2]:
+            dy, dw = moe_combine_bwd(dout, y, pos, weights, group_sizes)
+        return dy, None, dw, None, dout if ctx.needs_input_grad[4] else None
+
+
+def moe_combine(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, group_sizes: torch.Tensor, *,
+                residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The experts' rows back to their tokens: out[t] = residual[t] + sum_j
+    weights[t, j] * y[pos[t, j]] (y bf16 or fp32 [rows, K], out bf16), summed in
+    fp32 and rounded once; for pos, weights and counts (group_sizes) of
+    moe_route.  Differentiable in y, weights and residual."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, residual)):
+        return _MoECombine.apply(y, pos, weights, group_sizes, residual)
+    return moe_combine_fwd(y, pos, weights, residual=residual)
+
+
 def device_status() -> int:
     """Synchronises the current stream and returns (and clears) the library's
     device error word: 0 when no kernel reported a problem."""

@@ -44,6 +44,7 @@ extern "C" {
 #define GL_DEV_OK 0
 #define GL_DEV_WAIT_TIMEOUT 1   /* an mbarrier wait exceeded its poll budget */
 #define GL_DEV_BAD_GROUPS 2     /* group_sizes sum exceeds M or a size < 0 */
+#define GL_DEV_BAD_INDEX 3      /* a row index is past the rows (the row is skipped) */
 
 /* Output dtypes of the grouped matmul. */
 #define GL_OUT_BF16 0
@@ -353,6 +354,89 @@ size_t gl_rms_norm_bwd_workspace_bytes(int64_t M, int64_t K);
 int gl_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int weight_f32,
                     const float* rstd, int64_t M, int64_t K, void* dx, void* dweight, void* workspace,
                     size_t workspace_bytes, int* err_word, void* stream);
+
+/* Largest topk of the router and of the exchange. */
+#define GL_MOE_MAX_TOPK 32
+
+/*
+ * Router in front of the grouped matmul.  No counterpart in the reference,
+ * whose templates take group_sizes as an input.
+ *   logits   [T, E] fp32 (logits_f32 != 0) or bf16, 1 <= E <= 1024
+ *   mask     bool [T] (one byte each, 0: the token takes no part) or NULL
+ *   ids      int32 [T, topk] experts of the topk largest logits, in falling
+ *            order, ties to the lowest expert; 1 <= topk <= min(E, 32)
+ *   weights  fp32 [T, topk] their softmax, over its sum with renormalize != 0
+ *   counts   int32 [E] choices of every expert: group_sizes of gl_gmm_fp8_fwd
+ *   pos      int32 [T, topk] row of a choice when all choices are sorted by
+ *            (expert, token, slot)
+ *   loss     fp32 [1] balance loss E * sum_e f_e P_e, f_e = counts_e /
+ *            sum(counts), P_e = the softmax's mean over the routed tokens (1
+ *            when both are even; 0 without tokens)
+ *   routed   fp32 [1] number of routed tokens, at least 1 (for the backward)
+ * A logit of -inf takes its expert out for that token; a token that the mask
+ * takes out, or whose logits are all -inf, is in no sum.  Slots without an
+ * expert have ids -1, pos -1 and weight 0.  A NaN logit is never chosen, it
+ * makes its token's weights and the loss NaN (so does +inf).
+ * T >= 0, T * topk <= 2^31 - 1.  workspace: gl_moe_route_workspace_bytes(T, E)
+ * bytes (0 for an unsupported shape), 4-byte aligned, not used by another call
+ * in flight.  err_word is accepted for symmetry and never written.
+ */
+size_t gl_moe_route_workspace_bytes(int64_t T, int64_t E);
+int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64_t T, int64_t E,
+                     int64_t topk, int renormalize, int32_t* ids, float* weights, int32_t* counts,
+                     int32_t* pos, float* loss, float* routed, void* workspace, size_t workspace_bytes,
+                     int* err_word, void* stream);
+
+/*
+ * Backward of gl_moe_route_fwd: dlogits [T, E] (of logits' type) for the
+ * gradients dweights fp32 [T, topk] and dloss fp32 [1] (device; either may be
+ * NULL: zero).  logits, mask, renormalize as the forward took them, ids,
+ * weights, counts and routed as it wrote them.  The choice and the counts are
+ * constants.  Tokens that were not routed get zeros.
+ */
+int gl_moe_route_bwd(const void* logits, int logits_f32, const void* mask, const int32_t* ids,
+                     const float* weights, const int32_t* counts, const float* routed,
+                     const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t topk,
+                     int renormalize, void* dlogits, int* err_word, void* stream);
+
+/*
+ * Rows into expert order: out[pos[t, j]] = x[t] for every pos >= 0.
+ *   x            [T, row_bytes] (any type; row_bytes a multiple of 16)
+ *   s            fp32 [T, scales] moved alongside into out_s, or both NULL
+ *   pos          int32 [T, topk] as gl_moe_route_fwd writes it: distinct rows
+ *                below sum(group_sizes); a negative one is skipped
+ *   group_sizes  int32 [G], 1 <= G <= 1024
+ *   out, out_s   [rows, ...]; rows at or past sum(group_sizes) are set to
+ *                zero, their scales to 1 (the pair of a zero block)
+ * A pos at or past rows is skipped and sets GL_DEV_BAD_INDEX; a negative size
+ * or a sum past rows sets GL_DEV_BAD_GROUPS and leaves the tail as it is.
+ * x and out 16-byte aligned; T * topk and rows <= 2^31 - 1.
+ */
+int gl_moe_dispatch(const void* x, int64_t row_bytes, const float* s, int64_t scales, const int32_t* pos,
+                    const int32_t* group_sizes, int64_t G, int64_t T, int64_t topk, int64_t rows, void* out,
+                    float* out_s, int* err_word, void* stream);
+
+/*
+ * Rows back to their tokens: out[t] = residual[t] + sum_j weights[t, j] *
+ * y[pos[t, j]] over pos >= 0, summed in fp32 in slot order, rounded once.
+ *   y         [rows, K] bf16, or fp32 with y_f32 != 0 (gl_gmm_fp8_fwd's out)
+ *   weights   fp32 [T, topk], NULL for 1 (the backward of gl_moe_dispatch)
+ *   residual  bf16 [T, K] or NULL;  out bf16 [T, K]
+ * K % 8 == 0, K <= 16384; y, residual and out 16-byte aligned.  A pos past
+ * rows is left out and sets GL_DEV_BAD_INDEX.
+ */
+int gl_moe_combine(const void* y, int y_f32, const int32_t* pos, const float* weights, const void* residual,
+                   int64_t T, int64_t topk, int64_t K, int64_t rows, void* out, int* err_word, void* stream);
+
+/*
+ * Backward of gl_moe_combine for dout bf16 [T, K] (residual's gradient is dout
+ * itself): dy [rows, K] of y's type, dy[pos[t, j]] = weights[t, j] * dout[t],
+ * rows at or past sum(group_sizes) zero; dweights fp32 [T, topk] =
+ * <dout[t], y[pos[t, j]]>, 0 where pos < 0.
+ */
+int gl_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t* pos, const float* weights,
+                       const int32_t* group_sizes, int64_t G, int64_t T, int64_t topk, int64_t K,
+                       int64_t rows, void* dy, float* dweights, int* err_word, void* stream);
 
 /* Largest M*K accepted by gl_gmm_fp8_act_fwd_noalloc (activation elements). */
 #define GL_NOALLOC_MAX_ACT_ELEMS (16u * 1024u * 1024u)
