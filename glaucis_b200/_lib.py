@@ -21,6 +21,7 @@ GL_EDEVICE = -3
 GL_OUT_BF16 = 0
 GL_OUT_F32 = 1
 GL_GLA_BF16_INTRA = 1
+GL_W4_ZERO_TAIL = 1
 DEV_CODES = {0: "ok", 1: "device wait timed out", 2: "invalid group_sizes (negative or sum > M)",
              3: "row index out of range"}
 
@@ -68,6 +69,10 @@ SIGNATURES = {
     "gl_moe_combine": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P]),
     "gl_moe_combine_bwd": (_I, [_P, _P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,
                                 _P]),
+    "gl_quant_w4_128x1": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "gl_gmm_w4_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "gl_gmm_w4_fwd": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I, _I, _P, ctypes.c_size_t,
+                           _P, _P]),
     "gl_device_status": (_I, [_P, _P, ctypes.POINTER(ctypes.c_int)]),
     "gl_last_error": (ctypes.c_char_p, []),
     "gl_version": (ctypes.c_char_p, []),

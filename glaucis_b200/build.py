@@ -21,7 +21,7 @@ LIB = PKG / "libglaucis_b200.so"
 
 SOURCES = ["capi.cu", "quant.cu", "gmm_fp8.cu", "chunk_gla.cu", "chunk_gla_bwd.cu",
            "gla_intermediates.cu", "noalloc.cu", "rms_norm.cu", "moe_route.cu",
-           "moe_exchange.cu"]
+           "moe_exchange.cu", "gmm_w4.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2",
               "--expt-relaxed-constexpr", "-Xptxas", "-v"]

@@ -87,6 +87,12 @@ int gl_launch_moe_combine_bwd(const void* dout, const void* y, int y_f32, const 
                               const float* weights, const int32_t* group_sizes, int64_t G, int64_t T,
                               int64_t k, int64_t K, int64_t rows, void* dy, float* dweights, int* err,
                               cudaStream_t st, int num_sms, const char** why);
+size_t gl_gmm_w4_ws_bytes(int64_t M, int64_t K);
+int gl_launch_gmm_w4(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
+                     int64_t M, int64_t K, int64_t N, void* out, int out_f32, int zero_tail, void* ws,
+                     int* err, cudaStream_t st, int num_sms, const char** why);
+int gl_launch_quant_w4(const void* w, int64_t G, int64_t K, int64_t N, void* q, float* s, cudaStream_t st,
+                       const char** why);
 
 namespace {
 
@@ -853,6 +859,62 @@ int gl_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t
                                            rows, dy, dweights, err_word ? err_word : d->err,
                                            static_cast<cudaStream_t>(stream), d->num_sms, &why);
   if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+// ---------------------------------------------------------------------------
+// 4-bit weights
+// ---------------------------------------------------------------------------
+static bool w4_shape_ok(int64_t M, int64_t K) {
+  return M >= 0 && M <= 0x7fffffff && K > 0 && K % 128 == 0 && K <= (int64_t(1) << 23);
+}
+
+int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, float* s, int* err_word,
+                      void* stream) {
+  (void)err_word;
+  const char* f = "gl_quant_w4_128x1";
+  if (!w || !w4 || !s) return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (G < 1 || G > 1024 || !w4_shape_ok(1, K) || N <= 0 || N % 32 != 0 || N > 0x7fffffff)
+    return fail(GL_EINVAL, std::string(f) + ": need 1 <= G <= 1024, K a multiple of 128 and N one of 32");
+  if (!aligned16(w) || !aligned16(w4) || !aligned16(s))
+    return fail(GL_EINVAL, std::string(f) + ": w, w4 and s must be 16-byte aligned");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  if (gl_launch_quant_w4(w, G, K, N, w4, s, static_cast<cudaStream_t>(stream), &why) != 0)
+    return fail(GL_ELAUNCH, std::string(f) + ": " + why);
+  return GL_OK;
+}
+
+size_t gl_gmm_w4_workspace_bytes(int64_t M, int64_t K) {
+  return w4_shape_ok(M, K) ? gl_gmm_w4_ws_bytes(M, K) : 0;
+}
+
+int gl_gmm_w4_fwd(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
+                  int64_t M, int64_t K, int64_t N, void* out, int out_dtype, int flags, void* workspace,
+                  size_t workspace_bytes, int* err_word, void* stream) {
+  const char* f = "gl_gmm_w4_fwd";
+  if (G < 1 || G > 1024) return fail(GL_EINVAL, std::string(f) + ": need 1 <= G <= 1024");
+  if (!w4_shape_ok(M, K) || N <= 0 || N % 32 != 0 || N > 0x7fffffff)
+    return fail(GL_EINVAL, std::string(f) + ": need M >= 0, K a multiple of 128 and N one of 32");
+  if (M / 8 + (M < G ? M : G) > 65535) return fail(GL_EINVAL, std::string(f) + ": too many rows");
+  if (out_dtype != GL_OUT_BF16 && out_dtype != GL_OUT_F32)
+    return fail(GL_EINVAL, std::string(f) + ": out_dtype must be GL_OUT_BF16 or GL_OUT_F32");
+  if (flags & ~GL_W4_ZERO_TAIL) return fail(GL_EINVAL, std::string(f) + ": unknown flags");
+  if (M == 0) return GL_OK;
+  if (!x || !w4 || !s || !group_sizes || !out) return fail(GL_EINVAL, std::string(f) + ": null pointer");
+  if (!aligned16(x) || !aligned16(w4) || !aligned16(s) || !aligned16(out) || !aligned16(workspace))
+    return fail(GL_EINVAL, std::string(f) + ": x, w4, s, out and the workspace must be 16-byte aligned");
+  if (!workspace || workspace_bytes < gl_gmm_w4_ws_bytes(M, K))
+    return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
+                                            "gl_gmm_w4_workspace_bytes gives");
+  DeviceState* d = nullptr;
+  if (int rc = device_state(&d)) return rc;
+  const char* why = "";
+  const int rc = gl_launch_gmm_w4(x, w4, s, group_sizes, G, M, K, N, out, out_dtype == GL_OUT_F32,
+                                  flags & GL_W4_ZERO_TAIL, workspace, err_word ? err_word : d->err,
+                                  static_cast<cudaStream_t>(stream), d->num_sms, &why);
+  if (rc != 0) return fail(rc == -1 ? GL_EINVAL : GL_ELAUNCH, std::string(f) + ": " + why);
   return GL_OK;
 }
 

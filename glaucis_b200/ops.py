@@ -1048,6 +1048,63 @@ def moe_combine(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, group
     return moe_combine_fwd(y, pos, weights, residual=residual)
 
 
+# ---------------------------------------------------------------------------
+# Grouped products with 4-bit weights, for few rows
+# ---------------------------------------------------------------------------
+def quant_w4_128x1(w: torch.Tensor, w4: Optional[torch.Tensor] = None,
+                   s: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """bf16 [G, K, N] -> (int32 [G, K/8, N], fp32 scales [G, K/128, N]): 4-bit
+    weights, eight along K in a word (nibble j of word [g, i, n] is q[g, 8i + j,
+    n] + 8, q in -7..7), one absmax scale per 128 weights of a column.  K a
+    multiple of 128, N of 32; `w4` / `s` may be given as preallocated outputs."""
+    with _same_device(w):
+        if w.dtype != torch.bfloat16 or w.dim() != 3:
+            raise ValueError("quant_w4_128x1 expects a 3-D bf16 tensor")
+        G, K, N = w.shape
+        w4 = _out(w4, (G, K // 8, N), torch.int32, w.device, "w4")
+        s = _out(s, (G, K // TILE, N), torch.float32, w.device, "s")
+        _lib.check(_lib.load().gl_quant_w4_128x1(w.data_ptr(), G, K, N, w4.data_ptr(), s.data_ptr(), None,
+                                                 _stream()), "gl_quant_w4_128x1")
+    return w4, s
+
+
+def gmm_w4_fwd(x: torch.Tensor, w4: torch.Tensor, s: torch.Tensor, group_sizes: torch.Tensor,
+               out_dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Grouped matmul of few rows with 4-bit weights: x bf16 [M, K] (rows in
+    group order), w4 and s as quant_w4_128x1 gives them, group_sizes int32 [G]
+    -> [M, N].  The decoding counterpart of gmm_fp8_fwd: reads half a byte a
+    weight of the groups that have rows, and x in bf16.  The weights are not
+    differentiated.  Rows at or beyond sum(group_sizes) are left as they are in
+    `out` (zeroed when allocated)."""
+    with _same_device(x, w4, s, group_sizes, out):
+        if x.dtype != torch.bfloat16 or x.dim() != 2:
+            raise ValueError("x must be a 2-D bf16 tensor")
+        M, K = x.shape
+        if w4.dtype != torch.int32 or w4.dim() != 3 or w4.shape[1] * 8 != K:
+            raise ValueError("w4 must be int32 [G, K/8, N]")
+        G, _, N = w4.shape
+        if s.dtype != torch.float32 or tuple(s.shape) != (G, K // TILE, N):
+            raise ValueError("s must be fp32 [G, K/128, N]")
+        if group_sizes.dtype != torch.int32 or group_sizes.numel() != G:
+            raise ValueError("group_sizes must be int32 [G]")
+        if out is None and out_dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("out_dtype must be bf16 or fp32")
+        if out is not None and (out.dtype not in (torch.bfloat16, torch.float32)
+                                or tuple(out.shape) != (M, N)):
+            raise ValueError("out must be a contiguous bf16 or fp32 [M, N] tensor")
+        flags = _lib.GL_W4_ZERO_TAIL if out is None else 0
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        code = _lib.GL_OUT_F32 if out.dtype == torch.float32 else _lib.GL_OUT_BF16
+        lib = _lib.load()
+        ws_bytes = lib.gl_gmm_w4_workspace_bytes(M, K)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.gl_gmm_w4_fwd(x.data_ptr(), w4.data_ptr(), s.data_ptr(), group_sizes.data_ptr(), G,
+                                     M, K, N, out.data_ptr(), code, flags, ws.data_ptr(), ws_bytes, None,
+                                     _stream()), "gl_gmm_w4_fwd")
+    return out
+
+
 def device_status() -> int:
     """Synchronises the current stream and returns (and clears) the library's
     device error word: 0 when no kernel reported a problem."""

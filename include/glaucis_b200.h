@@ -438,6 +438,43 @@ int gl_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t
                        const int32_t* group_sizes, int64_t G, int64_t T, int64_t topk, int64_t K,
                        int64_t rows, void* dy, float* dweights, int* err_word, void* stream);
 
+/* Flags of gl_gmm_w4_fwd. */
+#define GL_W4_ZERO_TAIL 1  /* rows at or past sum(group_sizes) are set to zero */
+
+/*
+ * Weight quantiser to 4 bits, one scale per 128 weights of a column.  No
+ * counterpart in the reference.
+ *   w   bf16 [G, K, N] row-major, K % 128 == 0, N % 32 == 0, G <= 1024
+ *   w4  int32 [G, K/8, N]: nibble j (bits 4j..4j+3) of word [g, i, n] is
+ *       q[g, 8i + j, n] + 8
+ *   s   fp32 [G, K/128, N], s = absmax(128 weights)/7 (1.0 when all are zero),
+ *       q = round-half-even(w / s), -7..7
+ * w, w4 and s 16-byte aligned.  err_word is accepted for symmetry.
+ */
+int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, float* s, int* err_word,
+                      void* stream);
+
+/*
+ * Grouped matmul of few rows (a decoding batch) with 4-bit weights:
+ *   out[m, n] = sum_b s[g, b, n] * sum_{k in block b} x[m, k] q[g, k, n]
+ * rows belonging to groups as in gl_gmm_fp8_fwd.
+ *   x   bf16 [M, K];  w4, s in gl_quant_w4_128x1's format, q in -8..7 (a
+ *       checkpoint's own scales will do);  group_sizes int32 [G] (device)
+ *   out [M, N] bf16 or fp32 (out_dtype); rows at or past sum(group_sizes) are
+ *       left as they are, or zeroed with GL_W4_ZERO_TAIL
+ * Products are exact, sums fp32.  A non-finite x makes its row's outputs
+ * non-finite.  K % 128 == 0, N % 32 == 0, 1 <= G <= 1024, M/8 + min(M, G) <=
+ * 65535; x, w4, s, out and the workspace 16-byte aligned.  The weights of a group are read once
+ * per 8 rows of it: the fp8 products are the better choice for many rows.
+ * workspace: gl_gmm_w4_workspace_bytes(M, K) bytes (0 for an unsupported
+ * shape), not used by another call in flight.  Negative sizes or a sum past M
+ * set GL_DEV_BAD_GROUPS (out is then unspecified).
+ */
+size_t gl_gmm_w4_workspace_bytes(int64_t M, int64_t K);
+int gl_gmm_w4_fwd(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
+                  int64_t M, int64_t K, int64_t N, void* out, int out_dtype, int flags, void* workspace,
+                  size_t workspace_bytes, int* err_word, void* stream);
+
 /* Largest M*K accepted by gl_gmm_fp8_act_fwd_noalloc (activation elements). */
 #define GL_NOALLOC_MAX_ACT_ELEMS (16u * 1024u * 1024u)
 
