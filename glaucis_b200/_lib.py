@@ -90,6 +90,8 @@ def lib_path() -> Path:
 def load(build_if_missing: bool = False):
     """Returns the loaded library, raising if the shared object is absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -67,7 +67,7 @@ size_t gl_rms_norm_bwd_ws_bytes(int64_t M, int64_t K, int num_sms);
 int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* weight, int w32,
                            const float* rstd, int64_t M, int64_t K, void* dx, void* dw, void* ws,
                            cudaStream_t st, int num_sms, const char** why);
-size_t gl_moe_route_ws_bytes(int64_t E);
+size_t gl_moe_route_ws_bytes(int64_t T, int64_t E);
 int gl_launch_moe_route_fwd(const void* logits, int f32, const void* mask, int64_t T, int64_t E, int64_t k,
                             int renorm, int32_t* ids, float* weights, int32_t* counts, int32_t* pos,
                             float* loss, float* routed, void* ws, cudaStream_t st, int num_sms,
@@ -737,7 +737,7 @@ static int route_check(const char* f, int64_t T, int64_t E, int64_t topk) {
 }
 
 size_t gl_moe_route_workspace_bytes(int64_t T, int64_t E) {
-  return route_shape_ok(T, E) ? gl_moe_route_ws_bytes(E) : 0;
+  return route_shape_ok(T, E) ? gl_moe_route_ws_bytes(T, E) : 0;
 }
 
 int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64_t T, int64_t E,
@@ -749,7 +749,8 @@ int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64
   if (int rc = route_check(f, T, E, topk)) return rc;
   if (!counts || !loss || !routed || (T != 0 && (!logits || !ids || !weights || !pos)))
     return fail(GL_EINVAL, std::string(f) + ": null pointer");
-  if (!workspace || workspace_bytes < gl_moe_route_ws_bytes(E))
+  const size_t ws_need = gl_moe_route_ws_bytes(T, E);
+  if (ws_need && (!workspace || workspace_bytes < ws_need))
     return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
                                             "gl_moe_route_workspace_bytes gives");
   if ((reinterpret_cast<uintptr_t>(workspace) & 3u) != 0)
@@ -758,7 +759,7 @@ int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64
   if (int rc = device_state(&d)) return rc;
   const char* why = "";
   const int rc = gl_launch_moe_route_fwd(logits, logits_f32 != 0, mask, T, E, topk, renormalize != 0, ids,
-                                         weights, counts, pos, loss, routed, workspace,
+                                         weights, counts, pos, loss, routed, ws_need ? workspace : nullptr,
                                          static_cast<cudaStream_t>(stream), d->num_sms, &why);
   if (rc != 0) return fail(GL_ELAUNCH, std::string(f) + ": " + why);
   return GL_OK;

@@ -164,9 +164,12 @@ struct CombineArgs {
   int* err;
 };
 
-template <bool kF32>
+// B choices of a token are loaded at a time, U vectors of a lane from each:
+// B U = 8 loads in flight a lane (4 of twice the size for fp32), which is what
+// reaches HBM's rate; a batch wider than topk would leave half of them empty
+// (16387 tokens, topk 2, K 4096: 132 us with B = 4, U = 2).
+template <bool kF32, int B, int U>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
-  constexpr int U = 2, B = 4;  // vectors of a lane, choices loaded at a time
   const int lane = threadIdx.x & 31;
   const int segs = (a.nvec + 32 * U - 1) / (32 * U);
   const int64_t units = a.T * segs, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
@@ -192,6 +195,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
       Vec8<kF32> v[B][U];
 #pragma unroll
       for (int j = 0; j < B; ++j) {
+        // lanes from topk on hold -1
         const int64_t p = __shfl_sync(FULL, own, (j0 + j) & 31);
         const bool in = j0 + j < a.k && p >= 0;
 #pragma unroll
@@ -312,6 +316,12 @@ unsigned warp_ctas(int64_t units, int num_sms) {
   return static_cast<unsigned>(n > 0 ? n : 1);
 }
 
+template <bool kF32, int B, int U>
+void combine(const CombineArgs& a, int num_sms, cudaStream_t st) {
+  const int64_t units = a.T * ((a.nvec + 32 * U - 1) / (32 * U));
+  combine_kernel<kF32, B, U><<<warp_ctas(units, num_sms), 256, 0, st>>>(a);
+}
+
 template <int V>
 void combine_bwd(const CombineBwdArgs& a, int f32, unsigned ctas, int threads, cudaStream_t st) {
   if (f32)
@@ -343,11 +353,12 @@ int gl_launch_moe_combine(const void* y, int y_f32, const int32_t* pos, const fl
   using namespace gl::moe;
   const CombineArgs a{y, pos, weights, static_cast<const uint4*>(residual), T, rows, static_cast<int>(k),
                       static_cast<int>(K / 8), static_cast<uint4*>(out), err};
-  const int64_t units = T * ((a.nvec + 63) / 64);
-  if (y_f32)
-    combine_kernel<true><<<warp_ctas(units, num_sms), 256, 0, st>>>(a);
+  if (k == 1)
+    y_f32 ? combine<true, 1, 4>(a, num_sms, st) : combine<false, 1, 8>(a, num_sms, st);
+  else if (k == 2)
+    y_f32 ? combine<true, 2, 2>(a, num_sms, st) : combine<false, 2, 4>(a, num_sms, st);
   else
-    combine_kernel<false><<<warp_ctas(units, num_sms), 256, 0, st>>>(a);
+    y_f32 ? combine<true, 4, 1>(a, num_sms, st) : combine<false, 4, 2>(a, num_sms, st);
   return launched(why);
 }
 

@@ -6,15 +6,17 @@
 //   P_e = mean of the softmax over the routed tokens;
 // and the gradient of the logits for gradients of the weights and the loss.
 //
-// A warp takes a token, lane l holding experts l, l + 32, ...: the softmax's
-// sums and the k rounds of the selection are warp reductions on registers.  A
-// round finds the largest key with one redux.max and its lowest expert with
-// one redux.min, so it is bound by the latency of these (E floats a token are
-// little to read).  Rows need the counts of all earlier tokens: each CTA takes
-// consecutive tokens and leaves its counts per expert, a second launch (not
-// needed when one CTA takes all tokens) adds up those of the CTAs before it
-// and ranks its choices in order.  Counts are integers and the loss's sums run
-// in a fixed order over warps and CTAs: results do not depend on timing.
+// A warp takes a token, lane l holding the V experts from l V on: the softmax's
+// sums and the k rounds of the selection are warp reductions on registers.
+// Each lane keeps the largest of its own keys, so a round is one redux.max, a
+// ballot whose lowest lane holds the lowest expert of that key, and a rescan of
+// the winner's V keys.  With E floats a token to read it is bound by issuing
+// these instructions, not by HBM.  Rows need the counts of all earlier tokens:
+// each CTA takes consecutive tokens and leaves its counts per expert, a second
+// launch (not needed when one CTA takes all tokens) adds up those of the CTAs
+// before it and ranks its choices in order.  Counts are integers and the
+// loss's sums run in a fixed order over warps and CTAs: results do not depend
+// on timing.
 #include "common.cuh"
 
 namespace gl {
@@ -34,6 +36,7 @@ struct Args {
   const uint8_t* mask;  // or null
   int64_t T;
   int E, k, f32, renorm;
+  int vec;              // rows may be read in vectors
   int64_t chunk;        // tokens of a CTA
   int* ids;
   float* weights;
@@ -41,9 +44,9 @@ struct Args {
   int* pos;
   float* loss;
   float* routed;        // routed tokens, as a float
-  int* hist;            // [CTAs, E]
-  float* psum;          // [CTAs, E]
-  int* live;            // [CTAs]
+  int* hist;            // [CTAs, E]     } of the first launch, for the second
+  float* psum;          // [CTAs, E]     }
+  int* live;            // [CTAs]        }
 };
 
 template <int V>
@@ -54,7 +57,7 @@ struct Shared {
   };
   int hist[32 * V];   // this CTA's counts, then the row of an expert's next choice
   int total[32 * V];
-  float red[32];
+  float red[2][32];
   int live;
 };
 
@@ -81,83 +84,149 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// Softmax numerators of a token's logits z (lane l: experts l + 32 i); returns
-// 1 / their sum.
+// The lane's V logits of token t (experts lane V .. lane V + V - 1), -inf past
+// the last expert and for a token that the mask takes out.
 template <int V>
-__device__ __forceinline__ float softmax(const float (&z)[V], float (&e)[V], float& zmax) {
-  float m = -INFINITY;
+__device__ __forceinline__ void load_token(const Args& a, int64_t t, float (&z)[V]) {
+  const int e0 = (threadIdx.x & 31) * V;
+  const bool kept = a.mask == nullptr || __ldg(a.mask + t) != 0;
+  const int64_t at = t * a.E + e0;
+  if (a.vec) {
+    const bool in = kept && e0 < a.E;  // V divides E: all of the lane's or none
+    if (a.f32) {
+      const float* p = static_cast<const float*>(a.logits) + at;
+      if constexpr (V == 1) {
+        z[0] = in ? __ldg(p) : -INFINITY;
+      } else if constexpr (V == 2) {
+        const float2 v = in ? __ldg(reinterpret_cast<const float2*>(p)) : make_float2(-INFINITY, -INFINITY);
+        z[0] = v.x;
+        z[1] = v.y;
+      } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) m = fmaxf(m, z[i]);
+        for (int i = 0; i < V; i += 4) {
+          const float4 v = in ? __ldg(reinterpret_cast<const float4*>(p + i))
+                              : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          z[i] = v.x;
+          z[i + 1] = v.y;
+          z[i + 2] = v.z;
+          z[i + 3] = v.w;
+        }
+      }
+    } else {
+      constexpr uint32_t kNegInf2 = 0xFF80FF80u;  // two bf16 -inf
+      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(a.logits) + at;
+      if constexpr (V == 1) {
+        z[0] = in ? __bfloat162float(__ldg(p)) : -INFINITY;
+      } else if constexpr (V < 8) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-  zmax = m;
+        for (int i = 0; i < V; i += 2) {
+          const uint32_t w = in ? __ldg(reinterpret_cast<const uint32_t*>(p + i)) : kNegInf2;
+          const float2 v = bf16x2_to_f32x2(w);
+          z[i] = v.x;
+          z[i + 1] = v.y;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 8) {
+          const uint4 u = in ? __ldg(reinterpret_cast<const uint4*>(p + i))
+                             : make_uint4(kNegInf2, kNegInf2, kNegInf2, kNegInf2);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 v = bf16x2_to_f32x2(w[j]);
+            z[i + 2 * j] = v.x;
+            z[i + 2 * j + 1] = v.y;
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = kept && e0 + i < a.E ? load_logit(a.logits, a.f32, at + i) : -INFINITY;
+  }
+}
+
+// A token takes part when a logit of it is not -inf (NaN takes part, to show).
+template <int V>
+__device__ __forceinline__ bool takes_part(const float (&z)[V]) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i) any = any || z[i] != -INFINITY;
+  return __any_sync(FULL, any);
+}
+
+// Largest of the lane's keys and where it is first.
+template <int V>
+__device__ __forceinline__ void own_max(const uint32_t (&key)[V], uint32_t& m, int& arg) {
+  m = key[0];
+  arg = 0;
+#pragma unroll
+  for (int i = 1; i < V; ++i)
+    if (key[i] > m) {
+      m = key[i];
+      arg = i;
+    }
+}
+
+// Softmax numerators e of the logits z; returns 1 / their sum.
+template <int V>
+__device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float (&e)[V]) {
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    e[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - m);
+    e[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - zmax);
     s += e[i];
   }
   return 1.0f / warp_sum(s);
 }
 
-// A token takes part when the mask keeps it and a logit of it is not -inf.
+// Routes tokens [t0, t1): ids, weights; counts into sh.hist, each warp's
+// softmax sums into sh.psum and the number of routed tokens into sh.live.
 template <int V>
-__device__ __forceinline__ bool load_token(const Args& a, int64_t t, float (&z)[V]) {
-  const int lane = threadIdx.x & 31;
-  const bool kept = a.mask == nullptr || __ldg(a.mask + t) != 0;
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = lane + 32 * i;
-    z[i] = e < a.E && kept ? load_logit(a.logits, a.f32, t * a.E + e) : -INFINITY;
-    any = any || z[i] != -INFINITY;
-  }
-  return __any_sync(FULL, any);
-}
-
-// Routes tokens [t0, t1): ids, weights; counts into sh.hist, softmax sums and
-// the number of routed tokens into the CTA's slots.
-template <int V>
-__device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& sh, int cta) {
+__device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) sh.hist[e] = 0;
   if (threadIdx.x == 0) sh.live = 0;
   __syncthreads();
-  float psum[V] = {};
+  float psum[V] = {}, next[V];
   int live = 0;
+  if (t0 + warp < t1) load_token<V>(a, t0 + warp, next);
   for (int64_t t = t0 + warp; t < t1; t += warps<V>()) {
-    float z[V], e[V], zmax;
-    const bool in = load_token<V>(a, t, z);
+    float z[V], e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = next[i];
+    if (t + warps<V>() < t1) load_token<V>(a, t + warps<V>(), next);
     int id = -1;
     float p = 0.0f;
-    if (in) {
+    if (takes_part<V>(z)) {
       ++live;
-      const float inv = softmax<V>(z, e, zmax);
-      uint32_t key[V];
+      uint32_t key[V], own, mine = 0;
+      int arg;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        psum[i] += e[i] * inv;
-        key[i] = key_of(z[i]);
-      }
-      for (int j = 0; j < a.k; ++j) {
-        uint32_t m = key[0];
+      for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
+      own_max<V>(key, own, arg);
+      uint32_t m = __reduce_max_sync(FULL, own);
+      const float zmax = m ? of_key(m) : -INFINITY;
+      const float inv = softmax<V>(z, zmax, e);
 #pragma unroll
-        for (int i = 1; i < V; ++i) m = max(m, key[i]);
-        m = __reduce_max_sync(FULL, m);
-        if (m == 0) break;  // nothing left to choose
-        uint32_t at = FULL;
-#pragma unroll
-        for (int i = V - 1; i >= 0; --i)
-          if (key[i] == m) at = static_cast<uint32_t>(lane + 32 * i);
-        at = __reduce_min_sync(FULL, at);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (at == static_cast<uint32_t>(lane + 32 * i)) key[i] = 0;
+      for (int i = 0; i < V; ++i) psum[i] = fmaf(e[i], inv, psum[i]);
+      for (int j = 0; m != 0; ) {  // 0: nothing left to choose
+        const int src = __ffs(__ballot_sync(FULL, own == m)) - 1;
+        const int at = __shfl_sync(FULL, lane * V + arg, src);
         if (lane == j) {
-          id = static_cast<int>(at);
-          p = expf(of_key(m) - zmax) * inv;
+          id = at;
+          mine = m;
         }
+        if (++j == a.k) break;
+        if (lane == src) {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (i == arg) key[i] = 0;
+          own_max<V>(key, own, arg);
+        }
+        m = __reduce_max_sync(FULL, own);
       }
+      if (id >= 0) p = expf(of_key(mine) - zmax) * inv;
       if (a.renorm) {
         const float s = warp_sum(p);
         if (id >= 0) p /= s;
@@ -170,17 +239,37 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& s
     }
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) sh.psum[warp][lane + 32 * i] = psum[i];
+  for (int i = 0; i < V; ++i) sh.psum[warp][lane * V + i] = psum[i];
   if (lane == 0 && live) atomicAdd(&sh.live, live);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
-    float s = 0.0f;
-#pragma unroll 8
-    for (int w = 0; w < warps<V>(); ++w) s += sh.psum[w][e];
-    a.psum[static_cast<int64_t>(cta) * a.E + e] = s;
-    a.hist[static_cast<int64_t>(cta) * a.E + e] = sh.hist[e];
+}
+
+// Exclusive scan of sh.total over the experts, added to sh.hist: warp 0, V
+// consecutive experts a lane.
+template <int V>
+__device__ __forceinline__ void add_scan(Shared<V>& sh) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int n[V], own = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      n[i] = sh.total[lane * V + i];
+      own += n[i];
+    }
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(FULL, inc, o);
+      if (lane >= o) inc += v;
+    }
+    int run = inc - own;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      sh.hist[lane * V + i] += run;
+      run += n[i];
+    }
   }
-  if (threadIdx.x == 0) a.live[cta] = sh.live;
+  __syncthreads();
 }
 
 // sh.total: choices of every expert; sh.hist: the first row of this CTA's
@@ -194,8 +283,9 @@ __device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
     const int e = i % (32 * V);
     if (e >= a.E) continue;
     int before = 0, total = 0;
+#pragma unroll 8
     for (int b = i / (32 * V); b < ctas; b += slices) {
-      const int h = a.hist[static_cast<int64_t>(b) * a.E + e];
+      const int h = __ldcg(a.hist + static_cast<int64_t>(b) * a.E + e);
       total += h;
       before += b < cta ? h : 0;
     }
@@ -203,26 +293,7 @@ __device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
     if (before) atomicAdd(&sh.hist[e], before);
   }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    // exclusive scan over the experts, V consecutive ones a lane
-    const int lane = threadIdx.x;
-    int own = 0;
-#pragma unroll 4
-    for (int i = 0; i < V; ++i) own += sh.total[lane * V + i];
-    int inc = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(FULL, inc, o);
-      if (lane >= o) inc += v;
-    }
-    int run = inc - own;
-#pragma unroll 4
-    for (int i = 0; i < V; ++i) {
-      sh.hist[lane * V + i] += run;
-      run += sh.total[lane * V + i];
-    }
-  }
-  __syncthreads();
+  add_scan<V>(sh);
 }
 
 // Rows of the choices of tokens [t0, t1), a batch of one choice a thread at a
@@ -233,11 +304,13 @@ __device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n0 = t0 * a.k, n1 = t1 * a.k;
   for (int64_t b = n0; b < n1; b += blockDim.x) {
+    const int64_t left = n1 - b;
+    const int used = left < blockDim.x ? static_cast<int>((left + 31) / 32) : warps<V>();
     uint32_t* zero = reinterpret_cast<uint32_t*>(&sh.cnt[0][0]);
-    for (int i = threadIdx.x; i < warps<V>() * 16 * V; i += blockDim.x) zero[i] = 0;
-    __syncthreads();
+    for (int i = threadIdx.x; i < used * 16 * V; i += blockDim.x) zero[i] = 0;
     const int64_t n = b + threadIdx.x;
     const int id = n < n1 ? a.ids[n] : -1;
+    __syncthreads();
     const uint32_t same = __match_any_sync(FULL, id);
     const int rank = __popc(same & ((1u << lane) - 1u));
     if (id >= 0 && rank == 0) sh.cnt[warp][id] = static_cast<uint16_t>(__popc(same));
@@ -245,7 +318,7 @@ __device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1
     for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
       int run = 0;
 #pragma unroll 8
-      for (int w = 0; w < warps<V>(); ++w) {
+      for (int w = 0; w < used; ++w) {
         const int c = sh.cnt[w][e];
         sh.cnt[w][e] = static_cast<uint16_t>(run);
         run += c;
@@ -259,53 +332,70 @@ __device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1
   }
 }
 
-// counts, the loss and the number of routed tokens (sh.total: all choices).
+// counts and the loss: sh.total are all choices of an expert, sh.psum[0..rows)
+// parts of the softmax's sum over `n` routed tokens.
 template <int V>
-__device__ void finish(const Args& a, Shared<V>& sh, int ctas) {
+__device__ void finish(const Args& a, Shared<V>& sh, int rows, int n) {
   float part = 0.0f, chosen = 0.0f;
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     float p = 0.0f;
-    for (int b = 0; b < ctas; ++b) p += a.psum[static_cast<int64_t>(b) * a.E + e];
-    a.counts[e] = sh.total[e];
-    part = fmaf(static_cast<float>(sh.total[e]), p, part);
-    chosen += static_cast<float>(sh.total[e]);
+#pragma unroll 8
+    for (int w = 0; w < rows; ++w) p += sh.psum[w][e];
+    const int c = sh.total[e];
+    a.counts[e] = c;
+    part = fmaf(static_cast<float>(c), p, part);
+    chosen += static_cast<float>(c);
   }
-  int n = 0;
-  for (int b = threadIdx.x & 31; b < ctas; b += 32) n += a.live[b];
-  n = __reduce_add_sync(FULL, n);
   part = warp_sum(part);
   chosen = warp_sum(chosen);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) {
+    sh.red[0][warp] = part;
+    sh.red[1][warp] = chosen;
+  }
   __syncthreads();
-  if (lane == 0) sh.red[warp] = part;
-  __syncthreads();
-  part = warp_sum(lane < warps<V>() ? sh.red[lane] : 0.0f);
-  __syncthreads();
-  if (lane == 0) sh.red[warp] = chosen;
-  __syncthreads();
-  chosen = warp_sum(lane < warps<V>() ? sh.red[lane] : 0.0f);
-  if (threadIdx.x == 0) {
-    const float tokens = static_cast<float>(max(n, 1));
-    *a.loss = static_cast<float>(a.E) * (part / fmaxf(chosen, 1.0f) / tokens);
-    *a.routed = tokens;
+  if (warp == 0) {
+    part = warp_sum(lane < warps<V>() ? sh.red[0][lane] : 0.0f);
+    chosen = warp_sum(lane < warps<V>() ? sh.red[1][lane] : 0.0f);
+    if (lane == 0) {
+      const float tokens = static_cast<float>(max(n, 1));
+      *a.loss = static_cast<float>(a.E) * (part / fmaxf(chosen, 1.0f) / tokens);
+      *a.routed = tokens;
+    }
   }
 }
 
-// kOne: a single CTA takes every token and finishes; else the first of two
-// launches.
-template <int V, bool kOne>
+// One CTA takes every token.
+template <int V>
+__global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a) {
+  __shared__ Shared<V> sh;
+  route_tokens<V>(a, 0, a.T, sh);
+  for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) {
+    sh.total[e] = sh.hist[e];
+    sh.hist[e] = 0;
+  }
+  __syncthreads();
+  finish<V>(a, sh, a.T < warps<V>() ? static_cast<int>(a.T) : warps<V>(), sh.live);
+  add_scan<V>(sh);
+  assign_rows<V>(a, sh, 0, a.T);
+}
+
+// First of two launches: the choices, and what the CTA adds to counts and loss.
+template <int V>
 __global__ void __launch_bounds__(32 * warps<V>()) route_kernel(const Args a) {
   __shared__ Shared<V> sh;
+  cudaTriggerProgrammaticLaunchCompletion();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
   const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
-  route_tokens<V>(a, t0, t1, sh, blockIdx.x);
-  if (kOne) {
-    __syncthreads();
-    first_rows<V>(a, sh, 1, 0);
-    finish<V>(a, sh, 1);
-    __syncthreads();
-    assign_rows<V>(a, sh, t0, t1);
+  route_tokens<V>(a, t0, t1, sh);
+  for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+    float s = 0.0f;
+#pragma unroll 8
+    for (int w = 0; w < warps<V>(); ++w) s += sh.psum[w][e];
+    a.psum[static_cast<int64_t>(blockIdx.x) * a.E + e] = s;
+    a.hist[static_cast<int64_t>(blockIdx.x) * a.E + e] = sh.hist[e];
   }
+  if (threadIdx.x == 0) a.live[blockIdx.x] = sh.live;
 }
 
 // Second launch: the CTAs of the first rank their choices, one more finishes.
@@ -316,7 +406,22 @@ __global__ void __launch_bounds__(32 * warps<V>()) rank_kernel(const Args a) {
   const int ctas = gridDim.x - 1, cta = blockIdx.x;
   first_rows<V>(a, sh, ctas, cta);
   if (cta == ctas) {
-    finish<V>(a, sh, ctas);
+    // the CTAs' softmax sums, in as many slices as there are threads for
+    const int slices = blockDim.x >= 32 * V ? blockDim.x / (32 * V) : 1;
+    for (int i = threadIdx.x; i < slices * 32 * V; i += blockDim.x) {
+      const int e = i % (32 * V);
+      float s = 0.0f;
+      if (e < a.E) {
+#pragma unroll 8
+        for (int b = i / (32 * V); b < ctas; b += slices) s += __ldcg(a.psum + static_cast<int64_t>(b) * a.E + e);
+      }
+      sh.psum[i / (32 * V)][e] = s;
+    }
+    int n = 0;
+    for (int b = threadIdx.x & 31; b < ctas; b += 32) n += __ldcg(a.live + b);
+    n = __reduce_add_sync(FULL, n);
+    __syncthreads();
+    finish<V>(a, sh, slices, n);
     return;
   }
   const int64_t t0 = static_cast<int64_t>(cta) * a.chunk;
@@ -341,6 +446,42 @@ __device__ __forceinline__ void store_logit(void* p, int f32, int64_t i, float v
     static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// The lane's V values of token t's row.
+template <int V>
+__device__ __forceinline__ void store_token(const Args& a, void* out, int64_t t, const float (&v)[V]) {
+  const int e0 = (threadIdx.x & 31) * V;
+  const int64_t at = t * a.E + e0;
+  if (a.vec && V > 1) {
+    if (e0 >= a.E) return;
+    if (a.f32) {
+      float* p = static_cast<float*>(out) + at;
+      if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+      } else if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4)
+          *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      }
+    } else {
+      __nv_bfloat16* p = static_cast<__nv_bfloat16*>(out) + at;
+      if constexpr (V >= 8) {
+#pragma unroll
+        for (int i = 0; i < V; i += 8)
+          *reinterpret_cast<uint4*>(p + i) =
+              make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                         pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7]));
+      } else if constexpr (V >= 2) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(p + i) = pack_bf16x2(v[i], v[i + 1]);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (e0 + i < a.E) store_logit(out, a.f32, at + i, v[i]);
+}
+
 // dlogit_e = p_e (c_e + sel_e - sum_e' p_e' (c_e' + sel_e')), c_e = dloss E f_e / n
 // for the loss and sel_e the weights' part on the chosen experts.
 template <int V>
@@ -349,7 +490,7 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
   float c[V], chosen = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane + 32 * i;
+    const int e = lane * V + i;
     c[i] = e < a.E ? static_cast<float>(__ldg(b.counts + e)) : 0.0f;
     chosen += c[i];
   }
@@ -360,23 +501,32 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
   const int64_t warps_all = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.T;
        t += warps_all) {
-    float z[V], e[V], zmax;
-    const bool in = load_token<V>(a, t, z);
-    if (!in) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (lane + 32 * i < a.E) store_logit(b.dlogits, a.f32, t * a.E + lane + 32 * i, 0.0f);
-      continue;
-    }
+    float z[V], e[V];
+    load_token<V>(a, t, z);
     int id = -1;
     float sel = 0.0f, w = 0.0f;
     if (lane < a.k) {
       id = __ldg(b.ids + t * a.k + lane);
-      if (id < 0 || id >= a.E) id = -1;
       w = __ldg(b.weights + t * a.k + lane);
-      sel = b.dweights && id >= 0 ? __ldg(b.dweights + t * a.k + lane) : 0.0f;
+      sel = b.dweights ? __ldg(b.dweights + t * a.k + lane) : 0.0f;
+      if (id < 0 || id >= a.E) {
+        id = -1;
+        sel = 0.0f;
+      }
     }
-    const float inv = softmax<V>(z, e, zmax);
+    if (!takes_part<V>(z)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = 0.0f;
+      store_token<V>(a, b.dlogits, t, e);
+      continue;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, key_of(z[i]));
+    m = __reduce_max_sync(FULL, m);
+    const float zmax = m ? of_key(m) : -INFINITY;
+    const float inv = softmax<V>(z, zmax, e);
+    // the chosen experts' share, in the lane that holds the choice
     const float p_sel = id >= 0 ? expf(load_logit(a.logits, a.f32, t * a.E + id) - zmax) * inv : 0.0f;
     if (a.renorm) {
       const float dot = warp_sum(id >= 0 ? sel * w : 0.0f);
@@ -391,9 +541,8 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
     }
     dot = warp_sum(dot);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (lane + 32 * i < a.E)
-        store_logit(b.dlogits, a.f32, t * a.E + lane + 32 * i, e[i] * (c[i] - dot));
+    for (int i = 0; i < V; ++i) e[i] *= c[i] - dot;
+    store_token<V>(a, b.dlogits, t, e);
     __syncwarp();
     // the chosen experts' values over those just written (other lanes' stores,
     // ordered by the warp's barrier)
@@ -402,6 +551,9 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
                   p_sel * (static_cast<float>(__ldg(b.counts + id)) * scale + sel - dot));
   }
 }
+
+// Warps of a forward CTA for E experts.
+int fwd_warps(int64_t E) { return E <= 256 ? warps<8>() : E <= 512 ? warps<16>() : warps<32>(); }
 
 // CTAs of the forward: one when its warps take every token in a few rounds
 // (a second launch costs more than those rounds), else one per SM at most.
@@ -419,10 +571,10 @@ int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
   a.chunk = a.T > 0 ? (a.T + ctas - 1) / ctas : 1;
   cudaError_t e;
   if (ctas == 1) {
-    route_kernel<V, true><<<1, 32 * warps<V>(), 0, st>>>(a);
+    route_one_kernel<V><<<1, 32 * warps<V>(), 0, st>>>(a);
     e = cudaGetLastError();
   } else {
-    route_kernel<V, false><<<ctas, 32 * warps<V>(), 0, st>>>(a);
+    route_kernel<V><<<ctas, 32 * warps<V>(), 0, st>>>(a);
     e = cudaGetLastError();
     if (e == cudaSuccess) {
       // launched while the first runs out; it waits for it on the device
@@ -457,9 +609,23 @@ int bwd(const Args& a, const BwdArgs& b, int num_sms, cudaStream_t st, const cha
 }  // namespace route
 }  // namespace gl
 
-// hist and psum of every CTA, then its number of routed tokens.
-size_t gl_moe_route_ws_bytes(int64_t E) {
-  return static_cast<size_t>(gl::route::MAX_CTAS) * (2 * static_cast<size_t>(E) + 1) * 4;
+static bool vectors(const void* logits, int f32, int64_t E, int v) {
+  const int64_t bytes = v * (f32 ? 4 : 2);
+  return E % v == 0 && reinterpret_cast<uintptr_t>(logits) % (bytes < 16 ? bytes : 16) == 0;
+}
+
+// Experts of a lane.
+static int lane_experts(int64_t E) {
+  int v = 1;
+  while (v * 32 < E) v *= 2;
+  return v;
+}
+
+// hist and psum of every CTA, then its number of routed tokens; none for one CTA.
+size_t gl_moe_route_ws_bytes(int64_t T, int64_t E) {
+  using namespace gl::route;
+  if (fwd_ctas(T, fwd_warps(E), MAX_CTAS) == 1) return 0;
+  return static_cast<size_t>(MAX_CTAS) * (2 * static_cast<size_t>(E) + 1) * 4;
 }
 
 // Launchers: 0 on a launch, -2 on a launch error (why set).
@@ -468,24 +634,7 @@ int gl_launch_moe_route_fwd(const void* logits, int f32, const void* mask, int64
                             float* loss, float* routed, void* ws, cudaStream_t st, int num_sms,
                             const char** why) {
   using namespace gl::route;
-  int* hist = static_cast<int*>(ws);
-  float* psum = reinterpret_cast<float*>(hist + MAX_CTAS * E);
-  int* live = reinterpret_cast<int*>(psum + MAX_CTAS * E);
-  const Args a{logits, static_cast<const uint8_t*>(mask), T, static_cast<int>(E), static_cast<int>(k), f32,
-               renorm, 0, ids, weights, counts, pos, loss, routed, hist, psum, live};
-  if (E <= 32) return fwd<1>(a, num_sms, st, why);
-  if (E <= 64) return fwd<2>(a, num_sms, st, why);
-  if (E <= 128) return fwd<4>(a, num_sms, st, why);
-  if (E <= 256) return fwd<8>(a, num_sms, st, why);
-  if (E <= 512) return fwd<16>(a, num_sms, st, why);
-  return fwd<32>(a, num_sms, st, why);
-}
-
-int gl_launch_moe_route_bwd(const void* logits, int f32, const void* mask, const int32_t* ids,
-                            const float* weights, const int32_t* counts, const float* routed,
-                            const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t k,
-                            int renorm, void* dlogits, cudaStream_t st, int num_sms, const char** why) {
-  using namespace gl::route;
+  const int v = lane_experts(E);
   Args a = {};
   a.logits = logits;
   a.mask = static_cast<const uint8_t*>(mask);
@@ -494,11 +643,50 @@ int gl_launch_moe_route_bwd(const void* logits, int f32, const void* mask, const
   a.k = static_cast<int>(k);
   a.f32 = f32;
   a.renorm = renorm;
+  a.vec = vectors(logits, f32, E, v);
+  a.ids = ids;
+  a.weights = weights;
+  a.counts = counts;
+  a.pos = pos;
+  a.loss = loss;
+  a.routed = routed;
+  if (ws) {
+    a.hist = static_cast<int*>(ws);
+    a.psum = reinterpret_cast<float*>(a.hist + MAX_CTAS * E);
+    a.live = reinterpret_cast<int*>(a.psum + MAX_CTAS * E);
+  }
+  switch (v) {
+    case 1: return fwd<1>(a, num_sms, st, why);
+    case 2: return fwd<2>(a, num_sms, st, why);
+    case 4: return fwd<4>(a, num_sms, st, why);
+    case 8: return fwd<8>(a, num_sms, st, why);
+    case 16: return fwd<16>(a, num_sms, st, why);
+    default: return fwd<32>(a, num_sms, st, why);
+  }
+}
+
+int gl_launch_moe_route_bwd(const void* logits, int f32, const void* mask, const int32_t* ids,
+                            const float* weights, const int32_t* counts, const float* routed,
+                            const float* dweights, const float* dloss, int64_t T, int64_t E, int64_t k,
+                            int renorm, void* dlogits, cudaStream_t st, int num_sms, const char** why) {
+  using namespace gl::route;
+  const int v = lane_experts(E);
+  Args a = {};
+  a.logits = logits;
+  a.mask = static_cast<const uint8_t*>(mask);
+  a.T = T;
+  a.E = static_cast<int>(E);
+  a.k = static_cast<int>(k);
+  a.f32 = f32;
+  a.renorm = renorm;
+  a.vec = vectors(logits, f32, E, v) && vectors(dlogits, f32, E, v);
   const BwdArgs b{ids, weights, counts, routed, dweights, dloss, dlogits};
-  if (E <= 32) return bwd<1>(a, b, num_sms, st, why);
-  if (E <= 64) return bwd<2>(a, b, num_sms, st, why);
-  if (E <= 128) return bwd<4>(a, b, num_sms, st, why);
-  if (E <= 256) return bwd<8>(a, b, num_sms, st, why);
-  if (E <= 512) return bwd<16>(a, b, num_sms, st, why);
-  return bwd<32>(a, b, num_sms, st, why);
+  switch (v) {
+    case 1: return bwd<1>(a, b, num_sms, st, why);
+    case 2: return bwd<2>(a, b, num_sms, st, why);
+    case 4: return bwd<4>(a, b, num_sms, st, why);
+    case 8: return bwd<8>(a, b, num_sms, st, why);
+    case 16: return bwd<16>(a, b, num_sms, st, why);
+    default: return bwd<32>(a, b, num_sms, st, why);
+  }
 }

@@ -21,8 +21,14 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle without building a Stream object (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _need_cuda(*ts: Optional[torch.Tensor]) -> None:
@@ -628,12 +634,20 @@ _NO_GUARD = contextlib.nullcontext()
 def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
     """Checks that every tensor is a contiguous one on `first`'s CUDA device;
     returns a context in which that device is the current one."""
-    _need_cuda(first, *rest)
-    dev = first.device
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError(f"all tensors of a call must be on one device, got {dev} and {t.device}")
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    dev = first.get_device() if first.is_cuda else -1
+    for t in (first, *rest):
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            _need_cuda(t)
+        if t.get_device() != dev:
+            raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
+    return _NO_GUARD if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _new(like: torch.Tensor, t: Optional[torch.Tensor], shape, dtype: torch.dtype, name: str) -> torch.Tensor:
+    """_out on `like`'s device."""
+    return like.new_empty(shape, dtype=dtype) if t is None else _out(t, shape, dtype, like.device, name)
 
 
 class RMSNormForward(NamedTuple):
@@ -684,10 +698,10 @@ def rms_norm_quant_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
         M, K = _rms_check(x, weight, residual)
         if h is not None and residual is None:
             raise ValueError("h goes with a residual")
-        q = _out(q, (M, K), FP8, x.device, "q")
-        s = _out(s, (M, K // TILE), torch.float32, x.device, "s")
+        q = _new(x, q, (M, K), FP8, "q")
+        s = _new(x, s, (M, K // TILE), torch.float32, "s")
         if residual is not None:
-            h = _out(h, (M, K), torch.bfloat16, x.device, "h")
+            h = _new(x, h, (M, K), torch.bfloat16, "h")
         _rms_norm(x, weight, eps, residual, h, None, q, s, None)
     return (q, s) if residual is None else (q, s, h)
 
@@ -704,13 +718,13 @@ def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
         M, K = _rms_check(x, weight, residual)
         if h is not None and residual is None:
             raise ValueError("h goes with a residual")
-        y = _out(y, (M, K), torch.bfloat16, x.device, "y")
-        h = _out(h, (M, K), torch.bfloat16, x.device, "h") if residual is not None else x
+        y = _new(x, y, (M, K), torch.bfloat16, "y")
+        h = _new(x, h, (M, K), torch.bfloat16, "h") if residual is not None else x
         q = s = None
         if output_quant:
-            q = torch.empty((M, K), dtype=FP8, device=x.device)
-            s = torch.empty((M, K // TILE), dtype=torch.float32, device=x.device)
-        rstd = torch.empty(M, dtype=torch.float32, device=x.device)
+            q = x.new_empty((M, K), dtype=FP8)
+            s = x.new_empty((M, K // TILE), dtype=torch.float32)
+        rstd = x.new_empty(M, dtype=torch.float32)
         _rms_norm(x, weight, eps, residual, h, y, q, s, rstd)
     return RMSNormForward(y, h, q, s, rstd)
 
@@ -730,7 +744,7 @@ def rms_norm_bwd(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: 
         dx = torch.empty_like(h)
         dw = torch.empty_like(weight)
         ws_bytes = lib.gl_rms_norm_bwd_workspace_bytes(M, K)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=h.device) if ws_bytes else None
+        ws = h.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         _lib.check(lib.gl_rms_norm_bwd(dy.data_ptr(), _ptr(dh), h.data_ptr(), weight.data_ptr(),
                                        weight.dtype == torch.float32, rstd.data_ptr(), M, K,
                                        dx.data_ptr(), dw.data_ptr(), _ptr(ws), ws_bytes, None,
@@ -810,20 +824,19 @@ def moe_route_fwd(logits: torch.Tensor, topk: int, *, mask: Optional[torch.Tenso
     E <= 1024, topk <= 32."""
     with _same_device(logits, mask):
         T, E = _route_check(logits, mask)
-        dev = logits.device
-        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
-        pos = torch.empty((T, topk), dtype=torch.int32, device=dev)
-        weights = torch.empty((T, topk), dtype=torch.float32, device=dev)
-        counts = torch.empty(E, dtype=torch.int32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        routed = torch.empty((), dtype=torch.float32, device=dev)
+        ids = logits.new_empty((T, topk), dtype=torch.int32)
+        pos = torch.empty_like(ids)
+        weights = torch.empty_like(ids, dtype=torch.float32)
+        counts = logits.new_empty(E, dtype=torch.int32)
+        loss = logits.new_empty((), dtype=torch.float32)
+        routed = torch.empty_like(loss)
         lib = _lib.load()
         ws_bytes = lib.gl_moe_route_workspace_bytes(T, E)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws = logits.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         _lib.check(lib.gl_moe_route_fwd(logits.data_ptr(), logits.dtype == torch.float32, _ptr(mask), T, E,
                                         topk, renormalize, ids.data_ptr(), weights.data_ptr(),
                                         counts.data_ptr(), pos.data_ptr(), loss.data_ptr(),
-                                        routed.data_ptr(), ws.data_ptr(), ws_bytes, None, _stream()),
+                                        routed.data_ptr(), _ptr(ws), ws_bytes, None, _stream()),
                    "gl_moe_route_fwd")
     return MoERouting(ids, weights, counts, pos, loss, routed, mask, renormalize)
 
@@ -909,7 +922,7 @@ def moe_dispatch_fwd(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tens
         if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() != 2 or x.shape[0] != T:
             raise ValueError("x must be bf16 or fp32 [T, K]")
         rows = T * topk if rows is None else int(rows)
-        out = _out(out, (rows, x.shape[1]), x.dtype, x.device, "out")
+        out = _new(x, out, (rows, x.shape[1]), x.dtype, "out")
         _dispatch(x, None, pos, group_sizes, rows, out, None)
     return out
 
@@ -928,8 +941,8 @@ def moe_dispatch_quant(q: torch.Tensor, s: torch.Tensor, pos: torch.Tensor, grou
         if s.dtype != torch.float32 or tuple(s.shape) != (T, q.shape[1] // TILE) or q.shape[1] % TILE:
             raise ValueError("s must be fp32 [T, K/128], K a multiple of 128")
         rows = T * topk if rows is None else int(rows)
-        out = _out(out, (rows, q.shape[1]), FP8, q.device, "out")
-        out_s = _out(out_s, (rows, s.shape[1]), torch.float32, q.device, "out_s")
+        out = _new(q, out, (rows, q.shape[1]), FP8, "out")
+        out_s = _new(q, out_s, (rows, s.shape[1]), torch.float32, "out_s")
         _dispatch(q, s, pos, group_sizes, rows, out, out_s)
     return out, out_s
 
@@ -949,7 +962,7 @@ def moe_dispatch_bwd(dout: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         T, _ = _pos_check(pos)
         if dout.dtype not in (torch.bfloat16, torch.float32) or dout.dim() != 2:
             raise ValueError("dout must be bf16 or fp32 [rows, K]")
-        dx = torch.empty((T, dout.shape[1]), dtype=torch.bfloat16, device=dout.device)
+        dx = dout.new_empty((T, dout.shape[1]), dtype=torch.bfloat16)
         _combine(dout, pos, None, None, dx)
     return dx
 
@@ -997,7 +1010,7 @@ def moe_combine_fwd(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, *
         if residual is not None and (residual.dtype != torch.bfloat16
                                      or tuple(residual.shape) != (T, y.shape[1])):
             raise ValueError("residual must be bf16 [T, K]")
-        out = _out(out, (T, y.shape[1]), torch.bfloat16, y.device, "out")
+        out = _new(y, out, (T, y.shape[1]), torch.bfloat16, "out")
         _combine(y, pos, weights, residual, out)
     return out
 
@@ -1061,8 +1074,8 @@ def quant_w4_128x1(w: torch.Tensor, w4: Optional[torch.Tensor] = None,
         if w.dtype != torch.bfloat16 or w.dim() != 3:
             raise ValueError("quant_w4_128x1 expects a 3-D bf16 tensor")
         G, K, N = w.shape
-        w4 = _out(w4, (G, K // 8, N), torch.int32, w.device, "w4")
-        s = _out(s, (G, K // TILE, N), torch.float32, w.device, "s")
+        w4 = _new(w, w4, (G, K // 8, N), torch.int32, "w4")
+        s = _new(w, s, (G, K // TILE, N), torch.float32, "s")
         _lib.check(_lib.load().gl_quant_w4_128x1(w.data_ptr(), G, K, N, w4.data_ptr(), s.data_ptr(), None,
                                                  _stream()), "gl_quant_w4_128x1")
     return w4, s
@@ -1094,11 +1107,11 @@ def gmm_w4_fwd(x: torch.Tensor, w4: torch.Tensor, s: torch.Tensor, group_sizes: 
             raise ValueError("out must be a contiguous bf16 or fp32 [M, N] tensor")
         flags = _lib.GL_W4_ZERO_TAIL if out is None else 0
         if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+            out = x.new_empty((M, N), dtype=out_dtype)
         code = _lib.GL_OUT_F32 if out.dtype == torch.float32 else _lib.GL_OUT_BF16
         lib = _lib.load()
         ws_bytes = lib.gl_gmm_w4_workspace_bytes(M, K)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
         _lib.check(lib.gl_gmm_w4_fwd(x.data_ptr(), w4.data_ptr(), s.data_ptr(), group_sizes.data_ptr(), G,
                                      M, K, N, out.data_ptr(), code, flags, ws.data_ptr(), ws_bytes, None,
                                      _stream()), "gl_gmm_w4_fwd")

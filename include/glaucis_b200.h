@@ -378,8 +378,8 @@ int gl_rms_norm_bwd(const void* dy, const void* dh, const void* h, const void* w
  * expert have ids -1, pos -1 and weight 0.  A NaN logit is never chosen, it
  * makes its token's weights and the loss NaN (so does +inf).
  * T >= 0, T * topk <= 2^31 - 1.  workspace: gl_moe_route_workspace_bytes(T, E)
- * bytes (0 for an unsupported shape), 4-byte aligned, not used by another call
- * in flight.  err_word is accepted for symmetry and never written.
+ * bytes (0 when few tokens need none, or for an unsupported shape), 4-byte
+ * aligned, not used by another call in flight.  err_word is accepted for symmetry and never written.
  */
 size_t gl_moe_route_workspace_bytes(int64_t T, int64_t E);
 int gl_moe_route_fwd(const void* logits, int logits_f32, const void* mask, int64_t T, int64_t E,

@@ -20,8 +20,8 @@ def _route(T=4, E=16, k=2, z=P, ids=P, counts=P, ws=P, n=1 << 30):
 @pytest.mark.parametrize("kw,msg", [
     (dict(T=-1), "T"), (dict(T=1 << 31), "T"), (dict(E=0), "E"), (dict(E=1025, k=1), "E"), (dict(k=0), "topk"),
     (dict(k=17), "topk"), (dict(E=64, k=33), "topk"), (dict(T=1 << 30, k=2), "31 bits"), (dict(z=None), "null"),
-    (dict(ids=None), "null"), (dict(counts=None), "null"), (dict(ws=None), "workspace"), (dict(n=16), "workspace"),
-    (dict(ws=ctypes.c_void_p(18)), "4-byte"),
+    (dict(ids=None), "null"), (dict(counts=None), "null"), (dict(T=5000, ws=None), "workspace"), (dict(T=5000, n=16), "workspace"),
+    (dict(T=5000, ws=ctypes.c_void_p(18)), "4-byte"),
 ])
 def test_route_rejects(kw, msg):
     assert _route(**kw) == _lib.GL_EINVAL and msg in _err(), _err()
@@ -30,7 +30,8 @@ def test_route_rejects(kw, msg):
 def test_route_workspace_and_backward():
     lib = _lib.load()
     assert lib.gl_moe_route_workspace_bytes(4, 0) == 0 and lib.gl_moe_route_workspace_bytes(4, 2000) == 0
-    assert lib.gl_moe_route_workspace_bytes(4, 128) >= 2 * 128 * 4
+    assert lib.gl_moe_route_workspace_bytes(5000, 128) >= 2 * 128 * 4
+    assert lib.gl_moe_route_workspace_bytes(4, 128) == 0  # one CTA takes them all
     bwd = lambda T, E, k, z: lib.gl_moe_route_bwd(z, 1, None, P, P, P, P, None, None, T, E, k, 1, P, None, None)  # noqa: E731
     assert bwd(4, 16, 20, P) == _lib.GL_EINVAL and "topk" in _err()
     assert bwd(4, 16, 2, None) == _lib.GL_EINVAL and "null" in _err()
