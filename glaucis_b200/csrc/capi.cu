@@ -87,7 +87,7 @@ int gl_launch_moe_combine_bwd(const void* dout, const void* y, int y_f32, const 
                               const float* weights, const int32_t* group_sizes, int64_t G, int64_t T,
                               int64_t k, int64_t K, int64_t rows, void* dy, float* dweights, int* err,
                               cudaStream_t st, int num_sms, const char** why);
-size_t gl_gmm_w4_ws_bytes(int64_t M, int64_t K);
+size_t gl_gmm_w4_ws_bytes(int num_sms);
 int gl_launch_gmm_w4(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
                      int64_t M, int64_t K, int64_t N, void* out, int out_f32, int zero_tail, void* ws,
                      int* err, cudaStream_t st, int num_sms, const char** why);
@@ -169,6 +169,7 @@ uint32_t elem_bytes(CUtensorMapDataType dt) {
     case CU_TENSOR_MAP_DATA_TYPE_UINT8: return 1;
     case CU_TENSOR_MAP_DATA_TYPE_BFLOAT16:
     case CU_TENSOR_MAP_DATA_TYPE_FLOAT16: return 2;
+    case CU_TENSOR_MAP_DATA_TYPE_INT32:
     case CU_TENSOR_MAP_DATA_TYPE_FLOAT32: return 4;
     default: return 0;
   }
@@ -867,7 +868,7 @@ int gl_moe_combine_bwd(const void* dout, const void* y, int y_f32, const int32_t
 // 4-bit weights
 // ---------------------------------------------------------------------------
 static bool w4_shape_ok(int64_t M, int64_t K) {
-  return M >= 0 && M <= 0x7fffffff && K > 0 && K % 128 == 0 && K <= (int64_t(1) << 23);
+  return M >= 0 && M <= 0x7fffffff && K > 0 && K % 128 == 0 && K <= (int64_t(1) << 20);
 }
 
 int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, float* s, int* err_word,
@@ -888,7 +889,9 @@ int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, 
 }
 
 size_t gl_gmm_w4_workspace_bytes(int64_t M, int64_t K) {
-  return w4_shape_ok(M, K) ? gl_gmm_w4_ws_bytes(M, K) : 0;
+  DeviceState* d = nullptr;
+  if (!w4_shape_ok(M, K) || M == 0 || device_state(&d)) return 0;
+  return gl_gmm_w4_ws_bytes(d->num_sms);
 }
 
 int gl_gmm_w4_fwd(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
@@ -898,19 +901,20 @@ int gl_gmm_w4_fwd(const void* x, const void* w4, const float* s, const int32_t* 
   if (G < 1 || G > 1024) return fail(GL_EINVAL, std::string(f) + ": need 1 <= G <= 1024");
   if (!w4_shape_ok(M, K) || N <= 0 || N % 32 != 0 || N > 0x7fffffff)
     return fail(GL_EINVAL, std::string(f) + ": need M >= 0, K a multiple of 128 and N one of 32");
-  if (M / 8 + (M < G ? M : G) > 65535) return fail(GL_EINVAL, std::string(f) + ": too many rows");
   if (out_dtype != GL_OUT_BF16 && out_dtype != GL_OUT_F32)
     return fail(GL_EINVAL, std::string(f) + ": out_dtype must be GL_OUT_BF16 or GL_OUT_F32");
   if (flags & ~GL_W4_ZERO_TAIL) return fail(GL_EINVAL, std::string(f) + ": unknown flags");
+  if (M > 65536) return fail(GL_EINVAL, std::string(f) + ": too many rows (65536 at most)");
   if (M == 0) return GL_OK;
   if (!x || !w4 || !s || !group_sizes || !out) return fail(GL_EINVAL, std::string(f) + ": null pointer");
   if (!aligned16(x) || !aligned16(w4) || !aligned16(s) || !aligned16(out) || !aligned16(workspace))
     return fail(GL_EINVAL, std::string(f) + ": x, w4, s, out and the workspace must be 16-byte aligned");
-  if (!workspace || workspace_bytes < gl_gmm_w4_ws_bytes(M, K))
-    return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
-                                            "gl_gmm_w4_workspace_bytes gives");
+  if (!workspace) return fail(GL_EINVAL, std::string(f) + ": the workspace is missing");
   DeviceState* d = nullptr;
   if (int rc = device_state(&d)) return rc;
+  if (workspace_bytes < gl_gmm_w4_ws_bytes(d->num_sms))
+    return fail(GL_EINVAL, std::string(f) + ": the workspace is smaller than "
+                                            "gl_gmm_w4_workspace_bytes gives");
   const char* why = "";
   const int rc = gl_launch_gmm_w4(x, w4, s, group_sizes, G, M, K, N, out, out_dtype == GL_OUT_F32,
                                   flags & GL_W4_ZERO_TAIL, workspace, err_word ? err_word : d->err,

@@ -5,13 +5,25 @@
 // word w4[g, i, n] is k = 8 i + j.
 //
 // With few rows the product reads each weight of the groups in use once and
-// computes little with it: it is bound by HBM, and what must not get in the
-// way is the work of widening 4-bit weights.  So:
+// computes little with it: it is bound by HBM.  Three things must not get in
+// the way: the work of widening 4-bit weights, gaps in the stream of loads, and
+// what a call does before its first load.
+//   * One launch.  A persistent CTA takes an equal share of all (tile of 8
+//     rows, 512 columns, 128 k) units, cut at any k, so no SM waits for another
+//     one's longer list.  One thread copies weights and scales of the units
+//     into a ring of shared-memory stages with TMA, running ahead across
+//     tiles; a warp per stage puts the rows of x beside them in fragment order
+//     (one warp for all of them held the product back); eight warps take 64
+//     columns each (with 32, what a unit costs besides its weights did).
+//   * Where a share ends inside a tile's k, its fp32 sums go to the workspace;
+//     when its share is done a warp counts its parts in, and whoever completes a
+//     job's count adds the parts in order: the result does not depend on which
+//     one that is, and nothing waits.  (Counting in at the job's end, amid the
+//     loads, stood in their queue: 6 us of 20 for one token.)
 //   * Weights go through mma.sync (m16n8k16, fp16 in, fp32 sums) as the 16-row
 //     operand, 8 rows of x as the 8 columns: enough rate for a memory-bound
-//     product, no shared memory, fragments straight from global loads.  (A
-//     tcgen05 tile has 128 rows of shared-memory operands that would have to
-//     be widened and written first.)
+//     product.  (A tcgen05 tile would need the weights widened and written back
+//     to shared memory first, and has 128 rows.)
 //   * A nibble is used as it lies in the word: masked, it is the fp16
 //     subnormal u * 2^-24 (or 16 u * 2^-24 four bits up), exact in the matrix
 //     unit.  Eight weights cost four ANDs and one shift.  The x that meets the
@@ -21,123 +33,51 @@
 //     a power of two that takes its largest value to [2^13, 2^14), which is
 //     exact (values 2^38 below the largest lose bits far under the sum's
 //     rounding), and scaled back where the block's fp32 sum meets the weights'
-//     scale.  A first small launch does this once for all groups' rows, in the
-//     order the fragments want; the product's CTAs start beside it, find their
-//     group and load their first weights before they wait for it.
+//     scale.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "tmap.h"
 
 namespace gl {
 namespace w4 {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int COLS = 32;  // columns of a CTA
-constexpr int ROWS = 8;   // rows of a tile
-
-struct PrepArgs {
-  const uint4* x;
-  const int* sizes;
-  int64_t M;
-  int G, kb;         // kb: K / 128
-  uint4* xf;         // fp16 [M, K], each 8 in the order 0 4 1 5 2 6 3 7, odd ones / 16
-  float2* xs;        // [M, K / 128]: -8 * 2^-24 * sum of the scaled x, 2^(e + 12)
-  void* out;         // rows of no group are zeroed when zero_tail
-  int64_t row_words; // 16-byte words of an output row
-  int zero_tail;
-  int* err;
-};
-
-// 16 threads take a 128-block of a row.
-__global__ void __launch_bounds__(256) w4_prep_kernel(const PrepArgs a) {
-  cudaTriggerProgrammaticLaunchCompletion();
-  const int64_t blocks = a.M * a.kb;
-  const int sub = threadIdx.x & 15;
-  for (int64_t b0 = static_cast<int64_t>(blockIdx.x) * 16; b0 < blocks;
-       b0 += static_cast<int64_t>(gridDim.x) * 16) {
-    const int64_t b = b0 + (threadIdx.x >> 4);
-    const bool in = b < blocks;
-    const uint4 v = in ? __ldg(a.x + b * 16 + sub) : make_uint4(0, 0, 0, 0);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float f[8];
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 p = bf16x2_to_f32x2(w[i]);
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
-      m = fmaxf(m, fmaxf(fabsf(p.x), fabsf(p.y)));
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-    // exponent of the largest value, to 2^13; blocks below 2^-113 take 2^126
-    int e = static_cast<int>(__float_as_uint(m) >> 23) - 127 - 13;
-    e = e < -126 ? -126 : e;
-    const float scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] *= scale;
-      sum += f[i];
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
-    if (in) {
-      uint32_t h[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float d = i & 1 ? 0.0625f : 1.0f;
-        const __half2 p = __floats2half2_rn(f[i] * d, f[i + 4] * d);
-        h[i] = *reinterpret_cast<const uint32_t*>(&p);
-      }
-      a.xf[b * 16 + sub] = make_uint4(h[0], h[1], h[2], h[3]);
-      if (sub == 0)
-        a.xs[b] = make_float2(sum * -0x1p-21f, __uint_as_float(static_cast<uint32_t>(127 + e + 12) << 23));
-    }
-  }
-  // one CTA checks the sizes, all zero the rows of no group
-  __shared__ long long total;
-  __shared__ int bad;
-  if (threadIdx.x == 0) total = bad = 0;
-  __syncthreads();
-  long long own = 0;
-  for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    const int n = __ldg(a.sizes + g);
-    if (n < 0) bad = 1;
-    own += n;
-  }
-  if (own) atomicAdd(reinterpret_cast<unsigned long long*>(&total), static_cast<unsigned long long>(own));
-  __syncthreads();
-  if (bad || total > a.M) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(a.err, GL_DEV_BAD_GROUPS);
-    return;
-  }
-  if (a.zero_tail)
-    for (int64_t i = total * a.row_words + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-         i < a.M * a.row_words; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
-      static_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
-}
+constexpr int ROWS = 8;            // rows of a tile
+constexpr int COLS = 512;          // columns of a unit: 64 for each of the
+constexpr int WARPS = COLS / 64;   // consumer warps
+constexpr int STAGES = 3;          // two CTAs an SM
+constexpr int THREADS = 32 * (WARPS + 1 + STAGES);
+constexpr int MIN_UNITS = 2;       // a share is no smaller: a part's way through the workspace costs more
+// A stage: the weights as TMA leaves them, 32-column strips of 16 words a
+// column, 128-byte rows swizzled (16-byte chunk c of row r at c ^ (r & 7)); the
+// scales; the rows of x, 128 fp16 each (every 8 in the order 0 4 1 5 2 6 3 7,
+// odd ones / 16), then two floats (-8 * 2^-24 * sum of the scaled x, 2^(e + 12)).
+// In a 16-byte access phase lanes (gq, t), two gq and four t, read words 2 t +
+// const of the weights: chunks gq ^ (2 t + const) are eight different bank
+// groups, and so are rows of x 272 bytes apart.
+constexpr int S_OFF = COLS * 64;
+constexpr int X_OFF = S_OFF + COLS * 4;
+constexpr int X_BYTES = 272;
+constexpr int STAGE_BYTES = (X_OFF + ROWS * X_BYTES + 1023) / 1024 * 1024;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;  // aligned to 1 KB inside
 
 struct Args {
-  const uint4* w;      // [G, K / 8, N / 4] words of four columns
-  const float4* s;     // [G, K / 128, N / 4]
+  const uint4* x;
+  const float* s;      // [G, K / 128, N]
   const int* sizes;
-  const uint4* xf;
-  const float2* xs;
-  int64_t M;
-  int G, kb, n4;       // n4: N / 4
+  unsigned long long* tags;  // [CTAs, WARPS]: the call's number << 16, plus parts that are there
+  float* parts;              // [CTAs, 2, ROWS, COLS]
+  unsigned long long nonce;
+  int64_t M, N;
+  int G, kb, strips;   // kb: K / 128; strips: 512-column strips of N
   void* out;
-  int out_f32;
+  int out_f32, zero_tail;
+  int* err;
 };
-
-// Streaming 16-byte load: weights are read once, L1 is left to x.
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                     uint32_t b0, uint32_t b1) {
@@ -148,150 +88,538 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Group, first row and number of rows of tile `tile` (tiles of 8 rows, groups
-// in order); false when there are fewer.  A warp looks at 128 groups a step.
-__device__ __forceinline__ bool find_tile(const Args& a, int64_t tile, int& group, int64_t& row0, int& nrows) {
-  const int lane = threadIdx.x & 31;
-  int64_t rows_before = 0, tiles_before = 0;
-  for (int g0 = 0; g0 < a.G; g0 += 128) {
-    int n[4], rows = 0, tiles = 0;
+// The same with its own third operand.
+__device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+__device__ __forceinline__ uint4 lds4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float4 lds4f(uint32_t addr) {
+  const uint4 v = lds4(addr);
+  return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
+__device__ __forceinline__ float2 lds2f(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ unsigned long long atom_add_acq_rel(unsigned long long* p, unsigned long long v) {
+  unsigned long long old;
+  asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], %2;" : "=l"(old) : "l"(p), "l"(v) : "memory");
+  return old;
+}
+
+struct Tile {
+  int group, row0, nrows;
+};
+
+// The groups' rows and tiles (8 rows of one group), held by a warp: 128
+// groups a step, four consecutive ones a lane.  The step last looked at stays
+// in registers.
+struct Groups {
+  const int* sizes;
+  int G, M;
+  int n[4], rows, tiles;        // the lane's four groups; inclusive sums over the step's lanes
+  int rows_before, tiles_before, step;
+
+  // Sizes past M are held at M + 1: sums stay in 32 bits (M <= 2^16, G <= 2^10).
+  __device__ __forceinline__ bool load(int g0) {
+    const int lane = threadIdx.x & 31;
+    step = g0;
+    rows = tiles = 0;
+    bool bad = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int g = g0 + 4 * lane + j;
-      n[j] = g < a.G ? __ldg(a.sizes + g) : 0;
-      n[j] = n[j] < 0 ? 0 : n[j] > a.M ? static_cast<int>(a.M) : n[j];  // reported by the first launch
+      n[j] = g < G ? __ldg(sizes + g) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bad = bad || n[j] < 0;
+      n[j] = n[j] < 0 ? 0 : n[j] > M ? M + 1 : n[j];
       rows += n[j];
       tiles += (n[j] + ROWS - 1) / ROWS;
     }
-    int64_t r = rows, t = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t ro = __shfl_up_sync(FULL, r, o), to = __shfl_up_sync(FULL, t, o);
+      const int r = __shfl_up_sync(FULL, rows, o), t = __shfl_up_sync(FULL, tiles, o);
       if (lane >= o) {
-        r += ro;
-        t += to;
+        rows += r;
+        tiles += t;
       }
     }
-    const uint32_t past = __ballot_sync(FULL, tiles_before + t > tile);
-    if (past) {
-      const int src = __ffs(past) - 1;
-      int64_t r0 = rows_before + r - rows, t0 = tiles_before + t - tiles;
-      int g = 0, cnt = 0;
-      int64_t first = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int nt = (n[j] + ROWS - 1) / ROWS;
-        if (tile >= t0 && tile < t0 + nt) {
-          g = g0 + 4 * lane + j;
-          first = r0 + (tile - t0) * ROWS;
-          const int64_t left = r0 + n[j] - first;
-          cnt = static_cast<int>(left < ROWS ? left : ROWS);
-        }
-        t0 += nt;
-        r0 += n[j];
-      }
-      group = __shfl_sync(FULL, g, src);
-      row0 = __shfl_sync(FULL, first, src);
-      nrows = __shfl_sync(FULL, cnt, src);
-      return row0 + nrows <= a.M;
-    }
-    rows_before += __shfl_sync(FULL, r, 31);
-    tiles_before += __shfl_sync(FULL, t, 31);
+    return bad;
   }
-  return false;
+
+  // Number of tiles, and of rows; -1 when the sizes are not a partition of at
+  // most M rows.
+  __device__ __forceinline__ int count(int& total) {
+    bool bad = false;
+    rows_before = tiles_before = 0;
+    for (int g0 = 0;; g0 += 128) {
+      bad = load(g0) || bad;
+      const int r = rows_before + __shfl_sync(FULL, rows, 31), t = tiles_before + __shfl_sync(FULL, tiles, 31);
+      total = r;
+      if (g0 + 128 >= G) return __any_sync(FULL, bad) || r > M ? -1 : t;
+      rows_before = r;
+      tiles_before = t;
+    }
+  }
+
+  // Tile `want`, which exists.
+  __device__ __forceinline__ Tile find(int want) {
+    const int lane = threadIdx.x & 31;
+    if (want < tiles_before) {
+      rows_before = tiles_before = 0;
+      load(0);
+    }
+    while (want >= tiles_before + __shfl_sync(FULL, tiles, 31)) {
+      rows_before += __shfl_sync(FULL, rows, 31);
+      tiles_before += __shfl_sync(FULL, tiles, 31);
+      load(step + 128);
+    }
+    const int src = __ffs(__ballot_sync(FULL, want < tiles_before + tiles)) - 1;
+    int t0 = tiles_before + tiles, r0 = rows_before + rows;
+    Tile f = {0, 0, 0};
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      t0 -= (n[j] + ROWS - 1) / ROWS;
+      r0 -= n[j];
+      if (want >= t0 && want < t0 + (n[j] + ROWS - 1) / ROWS) {
+        const int in = (want - t0) * ROWS;
+        f.group = step + 4 * lane + j;
+        f.row0 = r0 + in;
+        f.nrows = n[j] - in < ROWS ? n[j] - in : ROWS;
+      }
+    }
+    f.group = __shfl_sync(FULL, f.group, src);
+    f.row0 = __shfl_sync(FULL, f.row0, src);
+    f.nrows = __shfl_sync(FULL, f.nrows, src);
+    return f;
+  }
+};
+
+// The equal shares: unit u = (tile * strips + strip) * kb + block belongs to
+// the CTA with start(c) <= u < start(c + 1); the first `longer` of them have
+// one unit more.
+struct Shares {
+  uint32_t each, longer, ctas;
+  __device__ __forceinline__ uint32_t start(uint32_t c) const { return c * each + (c < longer ? c : longer); }
+  __device__ __forceinline__ uint32_t owner(uint32_t u) const {
+    const uint32_t head = longer * (each + 1);
+    return u < head ? u / (each + 1) : longer + (u - head) / each;
+  }
+};
+
+// A CTA's share, unit by unit.
+struct Walk {
+  Groups groups;
+  Tile tile;
+  int job, block, at, strip;
+
+  __device__ __forceinline__ void begin(const Args& a, uint32_t u0) {
+    job = static_cast<int>(u0 / a.kb);
+    block = static_cast<int>(u0 - static_cast<uint32_t>(job) * a.kb);
+    at = job / a.strips;
+    strip = job - at * a.strips;
+    tile = groups.find(at);
+  }
+  // `more`: a further unit follows
+  __device__ __forceinline__ void advance(const Args& a, bool more) {
+    if (++block < a.kb) return;
+    block = 0;
+    ++job;
+    if (++strip < a.strips) return;
+    strip = 0;
+    if (more) tile = groups.find(++at);
+  }
+};
+
+struct Control {
+  uint64_t full[STAGES], empty[STAGES];
+  int rows[STAGES];  // rows of the stage's tile; negative where a job ends in this CTA
+  int4 job[STAGES];  // then: the job, the tile's first row, its strip
+  int4 part[2];      // row0, nrows, strip of the first and the last job, where the CTA has a part only
+  Shares shares;
+  int abort;
+};
+
+// The rows of x of one unit on their way to shared memory: half a warp a row,
+// eight features a lane.
+struct XRows {
+  uint4 v[ROWS / 2];
+
+  __device__ __forceinline__ void load(const Args& a, const Tile& tile, int block) {
+    const int half = (threadIdx.x >> 4) & 1, sub = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < ROWS / 2; ++i) {
+      const int r = 2 * i + half;
+      v[i] = r < tile.nrows
+                 ? __ldg(a.x + (static_cast<int64_t>(tile.row0 + r) * a.kb + block) * 16 + sub)
+                 : make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void store(uint32_t at, int nrows) const {
+    const int half = (threadIdx.x >> 4) & 1, sub = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < ROWS / 2; ++i) {
+      if (2 * i < nrows) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        float f[8], m = 0.0f, sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 p = bf16x2_to_f32x2(w[j]);
+          f[2 * j] = p.x;
+          f[2 * j + 1] = p.y;
+          m = fmaxf(m, fmaxf(fabsf(p.x), fabsf(p.y)));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+        // exponent of the largest value, to 2^13; blocks below 2^-113 take 2^126
+        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127 - 13;
+        e = e < -126 ? -126 : e;
+        const float scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f[j] *= scale;
+          sum += f[j];
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float d = j & 1 ? 0.0625f : 1.0f;
+          const __half2 p = __floats2half2_rn(f[j] * d, f[j + 4] * d);
+          h[j] = *reinterpret_cast<const uint32_t*>(&p);
+        }
+        const uint32_t row = at + (2 * i + half) * X_BYTES;
+        st_shared_v4(row + sub * 16, h[0], h[1], h[2], h[3]);
+        if (sub == 0)
+          st_shared_v4(row + 256, __float_as_uint(sum * -0x1p-21f), static_cast<uint32_t>(127 + e + 12) << 23, 0,
+                       0);
+      }
+    }
+  }
+};
+
+// The lane's sums as four pieces of four columns: piece e is row 2 t + (e & 1)
+// of half e >> 1 of the warp's columns.
+__device__ __forceinline__ float4 piece(const float (&tot)[4][4], int e) {
+  const int h = 2 * (e >> 1), o = e & 1;
+  return make_float4(tot[h][o], tot[h][2 + o], tot[h + 1][o], tot[h + 1][2 + o]);
 }
 
-// A CTA takes 32 columns of a tile; its W warps take the K blocks in turn and
-// add up through shared memory.  Lane (g, t) of a warp holds columns 4 g .. 4 g
-// + 3 and, of every 32 k, words (k / 8) t: four columns' words are one 16-byte
-// load, and one load of the warp covers four whole 128-byte lines.
-template <int W>
-__global__ void __launch_bounds__(32 * W) gmm_w4_kernel(const Args a) {
-  __shared__ float part[W][ROWS][COLS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, t = lane & 3;
-  int group = 0, nrows = 0;
-  int64_t row0 = 0;
-  if (!find_tile(a, blockIdx.y, group, row0, nrows)) {
-    cudaGridDependencySynchronize();  // the launch ends no earlier than the first one
-    return;
-  }
-  const int col4 = blockIdx.x * (COLS / 4) + gq;
-  const uint4* wp = a.w + (static_cast<int64_t>(group) * a.kb * 16 + t) * a.n4 + col4;
-  const float4* sp = a.s + static_cast<int64_t>(group) * a.kb * a.n4 + col4;
-  const uint4* xp = a.xf + (row0 + gq) * a.kb * 16 + t;
-  const float2* xsp = a.xs + (row0 + 2 * t) * a.kb;
-  const bool has_x = gq < nrows, r0 = 2 * t < nrows, r1 = 2 * t + 1 < nrows;
-  const int64_t line = 4 * static_cast<int64_t>(a.n4);  // 32 k further
+__device__ __forceinline__ void store4(const Args& a, int64_t row, int64_t col, const float4& v) {
+  const int64_t at = row * a.N + col;
+  if (a.out_f32)
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+  else
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
+        make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+}
 
-  uint4 nw[4];
-  float4 ns;
-  if (warp < a.kb) {
+__device__ __forceinline__ void write_out(const Args& a, const float (&tot)[4][4], int row0, int nrows, int strip) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) nw[i] = ld_stream(wp + (4 * warp + i) * line);
-    ns = __ldg(sp + static_cast<int64_t>(warp) * a.n4);
+  for (int e = 0; e < 4; ++e) {
+    const int r = 2 * (lane & 3) + (e & 1);
+    const int64_t col = static_cast<int64_t>(strip) * COLS + warp * 64 + 32 * (e >> 1) + 4 * (lane >> 2);
+    if (r < nrows && col < a.N) store4(a, row0 + static_cast<int64_t>(r), col, piece(tot, e));
   }
-  cudaGridDependencySynchronize();  // x in fragment order
+}
 
-  float tot[2][4] = {};
-  for (int kb = warp; kb < a.kb; kb += W) {
-    uint4 w[4];
+// Adds the parts of a job in the order of its CTAs: half a warp a row, four
+// columns a lane, P pairs of rows from C parts in flight.
+template <int P, int C>
+__device__ __forceinline__ void add_parts(const Args& a, const int4& job, uint32_t from, uint32_t to,
+                                          bool from_last) {
+  const int warp = threadIdx.x >> 5, r0 = (threadIdx.x >> 4) & 1, c4 = threadIdx.x & 15;
+  const int64_t col = static_cast<int64_t>(job.z) * COLS + warp * 64 + 4 * c4;
+  const float* q = a.parts + r0 * COLS + warp * 64 + 4 * c4;
+  float4 sum[P];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = nw[i];
-    const float4 s = ns;
-    uint4 x[4];
+  for (int j = 0; j < P; ++j) sum[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (uint32_t c0 = from; c0 <= to; c0 += C) {
+    float4 v[C][P];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = has_x ? __ldg(xp + kb * 16 + 4 * i) : make_uint4(0, 0, 0, 0);
-    const float2 xs0 = r0 ? __ldg(xsp + kb) : make_float2(0.0f, 0.0f);
-    const float2 xs1 = r1 ? __ldg(xsp + a.kb + kb) : make_float2(0.0f, 0.0f);
-    if (kb + W < a.kb) {
+    for (int i = 0; i < C; ++i) {
+      const uint32_t c = c0 + i;
+      // the part is the CTA's first; only the first of the job's CTAs can have
+      // begun with another job
+      const uint32_t slot = 2 * c + (c == from && from_last ? 1 : 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) nw[i] = ld_stream(wp + (4 * (kb + W) + i) * line);
-      ns = __ldg(sp + static_cast<int64_t>(kb + W) * a.n4);
-    }
-    float acc[2][4];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      acc[p][0] = acc[p][2] = xs0.x;
-      acc[p][1] = acc[p][3] = xs1.x;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t c[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint32_t u = c[2 * p], v = c[2 * p + 1];
-        mma(acc[p], u & 0x000F000Fu, v & 0x000F000Fu, u & 0x00F000F0u, v & 0x00F000F0u, x[i].x, x[i].y);
-        mma(acc[p], (u >> 8) & 0x000F000Fu, (v >> 8) & 0x000F000Fu, (u >> 8) & 0x00F000F0u,
-            (v >> 8) & 0x00F000F0u, x[i].z, x[i].w);
+      for (int j = 0; j < P; ++j) {
+        v[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (c <= to && r0 + 2 * j < job.y)
+          v[i][j] = __ldcg(reinterpret_cast<const float4*>(q + static_cast<int64_t>(slot) * (ROWS * COLS) +
+                                                           2 * j * COLS));
       }
     }
-    // 2^24 of the nibbles and 2^e of x, 12 of them on the scale: neither
-    // product leaves fp32's range before the other factor brings it back
-    const float sc[4] = {s.x * 4096.0f, s.y * 4096.0f, s.z * 4096.0f, s.w * 4096.0f};
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      tot[p][0] = fmaf(acc[p][0] * sc[2 * p], xs0.y, tot[p][0]);
-      tot[p][1] = fmaf(acc[p][1] * sc[2 * p], xs1.y, tot[p][1]);
-      tot[p][2] = fmaf(acc[p][2] * sc[2 * p + 1], xs0.y, tot[p][2]);
-      tot[p][3] = fmaf(acc[p][3] * sc[2 * p + 1], xs1.y, tot[p][3]);
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        sum[j].x += v[i][j].x;
+        sum[j].y += v[i][j].y;
+        sum[j].z += v[i][j].z;
+        sum[j].w += v[i][j].w;
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+    if (r0 + 2 * j < job.y && col < a.N) store4(a, job.x + static_cast<int64_t>(r0 + 2 * j), col, sum[j]);
+}
+
+__global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constant__ CUtensorMap wmap,
+                                                            const Args a) {
+  constexpr int S = STAGES;
+  extern __shared__ char smem_raw[];
+  __shared__ Control ct;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Abort ab{&ct.abort, a.err};
+  Walk walk;
+  if (warp >= WARPS) {
+    walk.groups.sizes = a.sizes;
+    walk.groups.G = a.G;
+    walk.groups.M = static_cast<int>(a.M);
+    int total = 0;
+    const int tiles = walk.groups.count(total);
+    if (warp == WARPS) {
+      if (lane == 0) {
+        prefetch_tmap(&wmap);
+        ct.abort = 0;
+        const uint32_t units = tiles < 0 ? 0 : static_cast<uint32_t>(tiles) * a.strips * a.kb;
+        const uint32_t most = (units + MIN_UNITS - 1) / MIN_UNITS;
+        Shares sh;
+        sh.ctas = most < gridDim.x ? most : gridDim.x;
+        sh.each = sh.ctas ? units / sh.ctas : 0;
+        sh.longer = sh.ctas ? units - sh.each * sh.ctas : 0;
+        ct.shares = sh;
+        for (int i = 0; i < S; ++i) {
+          mbar_init(&ct.full[i], 2);
+          mbar_init(&ct.empty[i], WARPS);
+        }
+        fence_mbar_init();
+      }
+    } else if (tiles < 0) {
+      if (blockIdx.x == 0 && lane == 0) atomicExch(a.err, GL_DEV_BAD_GROUPS);
+    } else if (a.zero_tail) {
+      const int64_t words = a.N * (a.out_f32 ? 4 : 2) / 16;
+      for (int64_t i = total * words + static_cast<int64_t>(blockIdx.x) * 32 + lane; i < a.M * words;
+           i += static_cast<int64_t>(gridDim.x) * 32)
+        static_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
     }
   }
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    *reinterpret_cast<float2*>(&part[warp][2 * t][4 * gq + 2 * p]) = make_float2(tot[p][0], tot[p][2]);
-    *reinterpret_cast<float2*>(&part[warp][2 * t + 1][4 * gq + 2 * p]) = make_float2(tot[p][1], tot[p][3]);
-  }
   __syncthreads();
-  for (int i = threadIdx.x; i < nrows * COLS; i += 32 * W) {
-    const int r = i / COLS, c = i % COLS;
-    float v = 0.0f;
+  const Shares sh = ct.shares;
+  if (blockIdx.x >= sh.ctas) return;
+  const uint32_t u0 = sh.start(blockIdx.x);
+  const int units = static_cast<int>(sh.start(blockIdx.x + 1) - u0);
+
+  if (warp == WARPS) {
+    // ---- weights and scales, and the stage's control words ----
+    walk.begin(a, u0);
+    int st = 0, n = 0;
+    uint32_t phase = 1;  // the first round of stages is free
+    for (; n < units; ++n) {
+      if (n >= S && !mbar_wait(&ct.empty[st], phase, ab)) break;
+      if (lane == 0) {
+        const Tile& tile = walk.tile;
+        const int64_t n0 = static_cast<int64_t>(walk.strip) * COLS;
+        const uint32_t bytes = static_cast<uint32_t>((a.N - n0 < COLS ? a.N - n0 : COLS) * 4);
+        const bool ends = walk.block == a.kb - 1 || n == units - 1;
+        ct.rows[st] = ends ? -tile.nrows : tile.nrows;
+        if (ends) ct.job[st] = make_int4(walk.job, tile.row0, walk.strip, 0);
+        mbar_arrive_expect_tx(&ct.full[st], S_OFF + bytes);
+        char* dst = smem_raw + (smem - smem_u32(smem_raw)) + st * STAGE_BYTES;
+        const int64_t kb = static_cast<int64_t>(tile.group) * a.kb + walk.block;
+        // columns past N are filled with zeros and counted
+        tma_load_3d(dst, &wmap, &ct.full[st], 0, static_cast<int>(kb * 16), walk.strip * (COLS / 32));
+        bulk_load(dst + S_OFF, a.s + kb * a.N + n0, bytes, &ct.full[st]);
+      }
+      walk.advance(a, n + 1 < units);
+      if (++st == S) {
+        st = 0;
+        phase ^= 1;
+      }
+    }
+    // the copies land before the CTA may end, also when it gives up
+    for (int i = n > S ? n - S : 0; i < n; ++i) {
+      const uint64_t from = global_ns();
+      while (!mbar_test(&ct.full[i % S], (i / S) & 1) && global_ns() - from < kWaitNs) {
+      }
+    }
+    return;
+  }
+
+  if (warp > WARPS) {
+    // ---- rows of x: a warp takes the units of one stage, the next one's rows
+    // loaded before this one's are stored ----
+    const int st = warp - WARPS - 1;
+    if (st >= units) return;
+    walk.begin(a, u0);
+    for (int i = 0; i < st; ++i) walk.advance(a, true);
+    XRows cur;
+    cur.load(a, walk.tile, walk.block);
+    uint32_t phase = 1;  // the first round is free
+    for (int n = st; n < units; n += S) {
+      const int nrows = walk.tile.nrows;
+      XRows next;
+      if (n + S < units) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) v += part[k][r][c];
-    const int64_t at = (row0 + r) * a.n4 * 4 + static_cast<int64_t>(blockIdx.x) * COLS + c;
-    if (a.out_f32)
-      static_cast<float*>(a.out)[at] = v;
+        for (int i = 0; i < S; ++i) walk.advance(a, true);
+        next.load(a, walk.tile, walk.block);
+      }
+      if (n >= S && !mbar_wait(&ct.empty[st], phase, ab)) return;
+      cur.store(smem + st * STAGE_BYTES + X_OFF, nrows);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ct.full[st]);
+      cur = next;
+      phase ^= 1;
+    }
+    return;
+  }
+
+  // ---- consumers: 64 columns a warp; lane (gq, t) holds columns 4 gq .. 4 gq
+  // + 3 of each half and four of the words k / 8 ----
+  const int gq = lane >> 2, t = lane & 3;
+  const uint32_t w_even = warp * 4096 + sw128_off(2 * t, gq), w_odd = warp * 4096 + sw128_off(2 * t + 1, gq);
+  const uint32_t s_at = S_OFF + warp * 256 + gq * 16, x_at = X_OFF + gq * X_BYTES + t * 32;
+  const uint32_t xs_at = X_OFF + 2 * t * X_BYTES + 256;
+  // The jobs of which this CTA may have a part only, its first (lane 0) and its
+  // last (lane 1), and the counts of their parts.  A count is taken over for
+  // this call by whoever comes first; each of a job's CTAs looks before it adds
+  // to it, so what the workspace held before does not matter, and the last one
+  // clears it for a replayed call, whose number is the same.
+  const uint32_t first_job = u0 / a.kb, last_job = (u0 + units - 1) / a.kb;
+  const uint32_t own_job = lane == 0 ? first_job : last_job;
+  const uint32_t own_from = sh.owner(own_job * a.kb), own_to = sh.owner(own_job * a.kb + a.kb - 1);
+  const bool own_split = own_from != own_to && (lane == 0 || (lane == 1 && last_job != first_job));
+  unsigned long long* const own_tag = a.tags + own_from * WARPS + warp;
+  if (own_split) {
+    unsigned long long old = *reinterpret_cast<volatile unsigned long long*>(own_tag);
+    while (old >> 16 != a.nonce) {
+      const unsigned long long seen = atomicCAS(own_tag, old, a.nonce << 16);
+      if (seen == old) break;
+      old = seen;
+    }
+  }
+  __syncwarp();
+  const bool split0 = __shfl_sync(FULL, own_split, 0), split1 = __shfl_sync(FULL, own_split, 1);
+  float tot[4][4] = {};  // [column pair][row 2t, 2t + 1 of either column]
+  int st = 0;
+  uint32_t phase = 0;
+  for (int n = 0; n < units; ++n) {
+    if (!mbar_wait(&ct.full[st], phase, ab)) return;
+    const int meta = ct.rows[st];
+    const uint32_t p = smem + st * STAGE_BYTES;
+    uint4 w[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      w[h][0] = lds4(p + w_even + h * 2048);
+      w[h][1] = lds4(p + w_odd + h * 2048);
+      w[h][2] = lds4(p + w_even + h * 2048 + 1024);
+      w[h][3] = lds4(p + w_odd + h * 2048 + 1024);
+    }
+    const float4 s0 = lds4f(p + s_at), s1 = lds4f(p + s_at + 128);
+    // 2^24 of the nibbles and 2^e of x, 12 of them on the scale: neither
+    // product leaves fp32's range before the other factor brings it back
+    const float sc[8] = {s0.x * 4096.0f, s0.y * 4096.0f, s0.z * 4096.0f, s0.w * 4096.0f,
+                         s1.x * 4096.0f, s1.y * 4096.0f, s1.z * 4096.0f, s1.w * 4096.0f};
+    // Rows past the tile's hold what an earlier unit left: a column of the
+    // matrix unit's result depends on its own row of x alone, and theirs are
+    // not stored.
+    const uint4 x[4] = {lds4(p + x_at), lds4(p + x_at + 16), lds4(p + x_at + 128), lds4(p + x_at + 144)};
+    const float2 xs0 = lds2f(p + xs_at), xs1 = lds2f(p + xs_at + X_BYTES);
+    const float offset[4] = {xs0.x, xs1.x, xs0.x, xs1.x};
+    float acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t c[8] = {w[0][i].x, w[0][i].y, w[0][i].z, w[0][i].w,
+                             w[1][i].x, w[1][i].y, w[1][i].z, w[1][i].w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t l = c[2 * h], v = c[2 * h + 1];
+        if (i == 0)
+          mma(acc[h], offset, l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[0].x, x[0].y);
+        else
+          mma(acc[h], l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[i].x, x[i].y);
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const uint32_t l = c[2 * h] >> 8, v = c[2 * h + 1] >> 8;
+        mma(acc[h], l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[i].z, x[i].w);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      tot[h][0] = fmaf(acc[h][0] * sc[2 * h], xs0.y, tot[h][0]);
+      tot[h][1] = fmaf(acc[h][1] * sc[2 * h], xs1.y, tot[h][1]);
+      tot[h][2] = fmaf(acc[h][2] * sc[2 * h + 1], xs0.y, tot[h][2]);
+      tot[h][3] = fmaf(acc[h][3] * sc[2 * h + 1], xs1.y, tot[h][3]);
+    }
+    int4 job = make_int4(0, 0, 0, 0);
+    if (meta < 0) job = ct.job[st];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ct.empty[st]);
+    if (++st == S) {
+      st = 0;
+      phase ^= 1;
+    }
+    if (meta >= 0) continue;
+
+    // the job's end here: its output, or a part of it
+    const int nrows = -meta;
+    const bool is_first = static_cast<uint32_t>(job.x) == first_job;
+    if (is_first ? split0 : split1 && static_cast<uint32_t>(job.x) == last_job) {
+      const int slot = is_first ? 0 : 1;
+      if (lane == 0) ct.part[slot] = make_int4(job.y, nrows, job.z, 0);  // the same from every warp
+      float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (ROWS * COLS) + warp * 64 + 4 * gq;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (2 * t + (e & 1) < nrows)
+          __stcg(reinterpret_cast<float4*>(part + (2 * t + (e & 1)) * COLS + 32 * (e >> 1)), piece(tot, e));
+    } else {
+      write_out(a, tot, job.y, nrows, job.z);
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h) tot[h][0] = tot[h][1] = tot[h][2] = tot[h][3] = 0.0f;
+  }
+
+  // the share is done: its parts are counted in, after the warp's stores
+  __syncwarp();
+  int there = -1;
+  if (own_split) there = static_cast<int>(atom_add_acq_rel(own_tag, 1) & 0xFFFF);
+  const bool complete = own_split && there == static_cast<int>(own_to - own_from);
+  if (complete) *own_tag = 0;
+#pragma unroll
+  for (int l = 0; l < 2; ++l) {
+    if (!__shfl_sync(FULL, complete, l)) continue;
+    const uint32_t job = l == 0 ? first_job : last_job;
+    const uint32_t from = __shfl_sync(FULL, own_from, l), to = __shfl_sync(FULL, own_to, l);
+    const bool from_last = sh.start(from) / a.kb != job;
+    const int4 pj = ct.part[l];
+    if (pj.y <= 2)
+      add_parts<1, 12>(a, pj, from, to, from_last);
     else
-      static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+      add_parts<4, 3>(a, pj, from, to, from_last);
   }
 }
 
@@ -335,26 +663,27 @@ int launched(const char** why) {
   return -2;
 }
 
-template <int W>
-cudaError_t launch(const Args& a, unsigned tiles, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.n4 * 4 / COLS), tiles);
-  cfg.blockDim = dim3(32 * W);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, gmm_w4_kernel<W>, a);
+// CTAs of the product: two an SM.
+int ctas(int num_sms) { return 2 * num_sms; }
+
+// A number of its own for every call of the process (splitmix64, Steele et al. 2014, of a counter:
+// nothing that a workspace is likely to hold).
+unsigned long long next_nonce() {
+  static std::atomic<uint64_t> calls{0};
+  uint64_t z = calls.fetch_add(1, std::memory_order_relaxed) * 0x9E3779B97F4A7C15ull + 0xD1B54A32D192ED03ull;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  z ^= z >> 31;
+  return z >> 16 ? z >> 16 : 1;  // 48 bits
 }
 
 }  // namespace w4
 }  // namespace gl
 
-// x in fragment order, then two floats a 128-block.
-size_t gl_gmm_w4_ws_bytes(int64_t M, int64_t K) {
-  return static_cast<size_t>(M) * K * 2 + static_cast<size_t>(M) * (K / 128) * 8;
+// The tags and the parts of the shares.
+size_t gl_gmm_w4_ws_bytes(int num_sms) {
+  using namespace gl::w4;
+  return static_cast<size_t>(ctas(num_sms)) * (WARPS * sizeof(unsigned long long) + 2 * ROWS * COLS * sizeof(float));
 }
 
 // Launchers: 0 on a launch, -1 on a bad argument, -2 on a launch error (why set).
@@ -362,26 +691,24 @@ int gl_launch_gmm_w4(const void* x, const void* w4, const float* s, const int32_
                      int64_t M, int64_t K, int64_t N, void* out, int out_f32, int zero_tail, void* ws,
                      int* err, cudaStream_t st, int num_sms, const char** why) {
   using namespace gl::w4;
-  const int kb = static_cast<int>(K / 128);
-  uint4* xf = static_cast<uint4*>(ws);
-  float2* xs = reinterpret_cast<float2*>(xf + M * (K / 8));
-  const PrepArgs p{static_cast<const uint4*>(x), group_sizes, M, static_cast<int>(G), kb, xf, xs, out,
-                   N * (out_f32 ? 4 : 2) / 16, zero_tail, err};
-  const int64_t need = (M * kb + 15) / 16, most = 4 * static_cast<int64_t>(num_sms);
-  w4_prep_kernel<<<static_cast<unsigned>(need < most ? need : most), 256, 0, st>>>(p);
-  if (const int rc = launched(why)) return rc;
-  const Args a{static_cast<const uint4*>(w4), reinterpret_cast<const float4*>(s), group_sizes, xf, xs, M,
-               static_cast<int>(G), kb, static_cast<int>(N / 4), out, out_f32};
-  // at most one short tile for every group that can have rows
-  const int64_t tiles = M / ROWS + (M < G ? M : G);
-  if (tiles > 65535) {
-    *why = "too many rows";
+  const int kb = static_cast<int>(K / 128), n = ctas(num_sms);
+  const int64_t strips = (N + COLS - 1) / COLS;
+  if ((M / ROWS + (M < G ? M : G)) * strips * kb > 0x7fffffff) {
+    *why = "too large a product";
     return -1;
   }
-  const cudaError_t e = launch<8>(a, static_cast<unsigned>(tiles), st);
-  if (e == cudaSuccess) return 0;
-  *why = cudaGetErrorString(e);
-  return -2;
+  // 32 columns x words x strips of 32 columns: a box is 16 strips of 16 words
+  CUtensorMap wmap;
+  if (!gl_make_tmap_3d(&wmap, CU_TENSOR_MAP_DATA_TYPE_INT32, w4, 32, G * (K / 8), N / 32, N, 32, 32, 16,
+                       COLS / 32, CU_TENSOR_MAP_SWIZZLE_128B, why))
+    return -1;
+  unsigned long long* tags = static_cast<unsigned long long*>(ws);
+  float* parts = reinterpret_cast<float*>(tags + n * WARPS);
+  const Args a{static_cast<const uint4*>(x), s, group_sizes, tags, parts, next_nonce(), M, N,
+               static_cast<int>(G), kb, static_cast<int>(strips), out, out_f32, zero_tail, err};
+  if (!gl_set_smem_attr(reinterpret_cast<const void*>(&gmm_w4_kernel), 0, SMEM_BYTES, why)) return -2;
+  gmm_w4_kernel<<<n, THREADS, SMEM_BYTES, st>>>(wmap, a);
+  return launched(why);
 }
 
 int gl_launch_quant_w4(const void* w, int64_t G, int64_t K, int64_t N, void* q, float* s, cudaStream_t st,

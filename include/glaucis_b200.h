@@ -463,11 +463,11 @@ int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, 
  *   out [M, N] bf16 or fp32 (out_dtype); rows at or past sum(group_sizes) are
  *       left as they are, or zeroed with GL_W4_ZERO_TAIL
  * Products are exact, sums fp32.  A non-finite x makes its row's outputs
- * non-finite.  K % 128 == 0, N % 32 == 0, 1 <= G <= 1024, M/8 + min(M, G) <=
- * 65535; x, w4, s, out and the workspace 16-byte aligned.  The weights of a group are read once
- * per 8 rows of it: the fp8 products are the better choice for many rows.
- * workspace: gl_gmm_w4_workspace_bytes(M, K) bytes (0 for an unsupported
- * shape), not used by another call in flight.  Negative sizes or a sum past M
+ * non-finite.  K % 128 == 0, N % 32 == 0, 1 <= G <= 1024, M <= 65536; x, w4, s,
+ * out and the workspace 16-byte aligned.  The weights of a group are read once per 32
+ * rows of it: gl_gmm_fp8_fwd is the better choice for many rows.
+ * workspace: gl_gmm_w4_workspace_bytes(M, K) bytes on the current device (0
+ * for an unsupported shape or M == 0), not used by another call in flight.  Negative sizes or a sum past M
  * set GL_DEV_BAD_GROUPS (out is then unspecified).
  */
 size_t gl_gmm_w4_workspace_bytes(int64_t M, int64_t K);
