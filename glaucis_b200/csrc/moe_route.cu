@@ -8,9 +8,9 @@
 //
 // A warp takes a token, lane l holding the V experts from l V on: the softmax's
 // sums and the k rounds of the selection are warp reductions on registers.
-// Each lane keeps the largest of its own keys, so a round is one redux.max, a
-// ballot whose lowest lane holds the lowest expert of that key, and a rescan of
-// the winner's V keys.  With E floats a token to read it is bound by issuing
+// Each lane keeps the largest of its own keys at hand, so a round is one
+// redux.max, a ballot whose lowest lane holds the lowest expert of that key,
+// and the winner's next key taking its place.  With E floats a token to read it is bound by issuing
 // these instructions, not by HBM.  Rows need the counts of all earlier tokens:
 // each CTA takes consecutive tokens and leaves its counts per expert, a second
 // launch (not needed when one CTA takes all tokens) adds up those of the CTAs
@@ -155,18 +155,9 @@ __device__ __forceinline__ bool takes_part(const float (&z)[V]) {
   return __any_sync(FULL, any);
 }
 
-// Largest of the lane's keys and where it is first.
-template <int V>
-__device__ __forceinline__ void own_max(const uint32_t (&key)[V], uint32_t& m, int& arg) {
-  m = key[0];
-  arg = 0;
-#pragma unroll
-  for (int i = 1; i < V; ++i)
-    if (key[i] > m) {
-      m = key[i];
-      arg = i;
-    }
-}
+// e^x for x <= 0 as 2^(x log2 e): two roundings of the exponent, |x| 2^-24
+// relative each, where subtracting the row's maximum already made one.
+__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.44269504f); }
 
 // Softmax numerators e of the logits z; returns 1 / their sum.
 template <int V>
@@ -174,11 +165,81 @@ __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float 
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    e[i] = z[i] == -INFINITY ? 0.0f : expf(z[i] - zmax);
+    e[i] = z[i] == -INFINITY ? 0.0f : exp_of(z[i] - zmax);
     s += e[i];
   }
-  return 1.0f / warp_sum(s);
+  return __fdividef(1.0f, warp_sum(s));  // the sum is 1 to 1024: within 2 ulp
 }
+
+// A lane's keys and where they are, so that the largest is at hand and the next
+// takes its place when it is chosen.  Up to four are kept sorted (equal keys in
+// the experts' order); of more, the largest is looked for again.
+template <int V>
+struct Keys {
+  static constexpr bool kSorted = V <= 4;
+  uint32_t key[V];
+  int at[V];  // kSorted: expert of each; else at[0]: index of the largest
+  uint32_t own;
+
+  __device__ __forceinline__ void order(int i, int j) {  // i < j
+    if (key[j] > key[i]) {
+      const uint32_t k = key[i];
+      key[i] = key[j];
+      key[j] = k;
+      const int t = at[i];
+      at[i] = at[j];
+      at[j] = t;
+    }
+  }
+  __device__ __forceinline__ void look() {
+    own = key[0];
+    at[0] = 0;
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (key[i] > own) {
+        own = key[i];
+        at[0] = i;
+      }
+  }
+  __device__ __forceinline__ void begin(const float (&z)[V]) {
+    const int e0 = (threadIdx.x & 31) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
+    if constexpr (kSorted) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) at[i] = e0 + i;
+      // insertion by neighbours only, which keeps equal keys in order
+#pragma unroll
+      for (int n = V - 1; n > 0; --n)
+#pragma unroll
+        for (int i = 0; i < n; ++i) order(i, i + 1);
+      own = key[0];
+    } else {
+      look();
+    }
+  }
+  __device__ __forceinline__ int expert() const {
+    if constexpr (kSorted) return at[0];
+    return (threadIdx.x & 31) * V + at[0];
+  }
+  // Takes the largest away (in the lane with `won`).
+  __device__ __forceinline__ void next(bool won) {
+    if constexpr (kSorted) {
+#pragma unroll
+      for (int i = 0; i + 1 < V; ++i) {
+        key[i] = won ? key[i + 1] : key[i];
+        at[i] = won ? at[i + 1] : at[i];
+      }
+      key[V - 1] = won ? 0 : key[V - 1];
+      own = key[0];
+    } else if (won) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == at[0]) key[i] = 0;
+      look();
+    }
+  }
+};
 
 // Routes tokens [t0, t1): ids, weights; counts into sh.hist, each warp's
 // softmax sums into sh.psum and the number of routed tokens into sh.live.
@@ -200,41 +261,34 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& s
     float p = 0.0f;
     if (takes_part<V>(z)) {
       ++live;
-      uint32_t key[V], own, mine = 0;
-      int arg;
-#pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
-      own_max<V>(key, own, arg);
-      uint32_t m = __reduce_max_sync(FULL, own);
+      Keys<V> keys;
+      keys.begin(z);
+      uint32_t m = __reduce_max_sync(FULL, keys.own), mine = 0;
       const float zmax = m ? of_key(m) : -INFINITY;
       const float inv = softmax<V>(z, zmax, e);
 #pragma unroll
       for (int i = 0; i < V; ++i) psum[i] = fmaf(e[i], inv, psum[i]);
       for (int j = 0; m != 0; ) {  // 0: nothing left to choose
-        const int src = __ffs(__ballot_sync(FULL, own == m)) - 1;
-        const int at = __shfl_sync(FULL, lane * V + arg, src);
+        const int src = __ffs(__ballot_sync(FULL, keys.own == m)) - 1;
+        const int at = __shfl_sync(FULL, keys.expert(), src);
         if (lane == j) {
           id = at;
           mine = m;
         }
         if (++j == a.k) break;
-        if (lane == src) {
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (i == arg) key[i] = 0;
-          own_max<V>(key, own, arg);
-        }
-        m = __reduce_max_sync(FULL, own);
+        keys.next(lane == src);
+        m = __reduce_max_sync(FULL, keys.own);
       }
-      if (id >= 0) p = expf(of_key(mine) - zmax) * inv;
+      if (id >= 0) p = exp_of(of_key(mine) - zmax) * inv;
       if (a.renorm) {
         const float s = warp_sum(p);
-        if (id >= 0) p /= s;
+        if (id >= 0) p = __fdividef(p, s);
       }
     }
     if (lane < a.k) {
-      a.ids[t * a.k + lane] = id;
-      a.weights[t * a.k + lane] = p;
+      const int n = static_cast<int>(t) * a.k + lane;  // T * topk fits 31 bits
+      a.ids[n] = id;
+      a.weights[n] = p;
       if (id >= 0) atomicAdd(&sh.hist[id], 1);
     }
   }
@@ -487,6 +541,19 @@ __device__ __forceinline__ void store_token(const Args& a, void* out, int64_t t,
 template <int V>
 __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdArgs b) {
   const int lane = threadIdx.x & 31;
+  // a token's logits and choices, read one token ahead
+  float next[V], w_next = 0.0f, sel_next = 0.0f;
+  int id_next = -1;
+  auto load = [&](int64_t t) {
+    load_token<V>(a, t, next);
+    if (lane < a.k) {
+      id_next = __ldg(b.ids + t * a.k + lane);
+      w_next = __ldg(b.weights + t * a.k + lane);
+      sel_next = b.dweights ? __ldg(b.dweights + t * a.k + lane) : 0.0f;
+    }
+  };
+  int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t < a.T) load(t);
   float c[V], chosen = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -499,21 +566,17 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
 #pragma unroll
   for (int i = 0; i < V; ++i) c[i] *= scale;
   const int64_t warps_all = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.T;
-       t += warps_all) {
+  for (; t < a.T; t += warps_all) {
     float z[V], e[V];
-    load_token<V>(a, t, z);
-    int id = -1;
-    float sel = 0.0f, w = 0.0f;
-    if (lane < a.k) {
-      id = __ldg(b.ids + t * a.k + lane);
-      w = __ldg(b.weights + t * a.k + lane);
-      sel = b.dweights ? __ldg(b.dweights + t * a.k + lane) : 0.0f;
-      if (id < 0 || id >= a.E) {
-        id = -1;
-        sel = 0.0f;
-      }
+#pragma unroll
+    for (int i = 0; i < V; ++i) z[i] = next[i];
+    int id = id_next;
+    float w = w_next, sel = sel_next;
+    if (id < 0 || id >= a.E) {
+      id = -1;
+      sel = 0.0f;
     }
+    if (t + warps_all < a.T) load(t + warps_all);
     if (!takes_part<V>(z)) {
 #pragma unroll
       for (int i = 0; i < V; ++i) e[i] = 0.0f;
@@ -527,7 +590,7 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
     const float zmax = m ? of_key(m) : -INFINITY;
     const float inv = softmax<V>(z, zmax, e);
     // the chosen experts' share, in the lane that holds the choice
-    const float p_sel = id >= 0 ? expf(load_logit(a.logits, a.f32, t * a.E + id) - zmax) * inv : 0.0f;
+    const float p_sel = id >= 0 ? exp_of(load_logit(a.logits, a.f32, t * a.E + id) - zmax) * inv : 0.0f;
     if (a.renorm) {
       const float dot = warp_sum(id >= 0 ? sel * w : 0.0f);
       const float s = warp_sum(p_sel);
@@ -598,7 +661,13 @@ int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
 template <int V>
 int bwd(const Args& a, const BwdArgs& b, int num_sms, cudaStream_t st, const char** why) {
   const int64_t need = (a.T + 7) / 8;
-  const int64_t most = static_cast<int64_t>(num_sms) * (V <= 8 ? 8 : 4);
+  int per_sm = 0;
+  cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, route_bwd_kernel<V>, 256, 0);
+  if (q != cudaSuccess) {
+    *why = cudaGetErrorString(q);
+    return -2;
+  }
+  const int64_t most = static_cast<int64_t>(num_sms) * per_sm;
   route_bwd_kernel<V><<<static_cast<unsigned>(need < most ? need : most), 256, 0, st>>>(a, b);
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return 0;

@@ -183,10 +183,12 @@ struct BwdArgs {
 };
 
 // A persistent CTA takes rows blockIdx.x, + gridDim.x, ... (kWarpRow: a warp
-// each) and keeps its columns' share of dw in registers.
-template <int V, bool kWarpRow>
-__global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
-    rms_norm_bwd_kernel(const BwdArgs a) {
+// each) and keeps its columns' share of dw in registers.  dy and h of the next
+// row are loaded while this row's sum is under way (where MAX_T leaves the
+// registers), dh, which only dx needs, with the row itself.
+template <int V, bool kWarpRow, int MAX_T, int CTAS>
+__global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs a) {
+  constexpr bool kAhead = MAX_T <= 512;
   __shared__ float part[2][32];
   __shared__ float cross[kWarpRow ? WARP_ROWS : 1][kWarpRow ? 32 * V * 8 : 1];
   const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
@@ -194,19 +196,31 @@ __global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
   const int64_t rows_step = kWarpRow ? static_cast<int64_t>(gridDim.x) * WARP_ROWS : gridDim.x;
   int64_t row = kWarpRow ? static_cast<int64_t>(blockIdx.x) * WARP_ROWS + (threadIdx.x >> 5)
                          : static_cast<int64_t>(blockIdx.x);
+  uint4 gn[V], hn[V];
+  auto load = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int vec = tid + i * step;
+      const bool in = r < a.M && vec < a.nvec;
+      gn[i] = in ? __ldg(a.dy + r * a.nvec + vec) : make_uint4(0, 0, 0, 0);
+      hn[i] = in ? __ldg(a.h + r * a.nvec + vec) : make_uint4(0, 0, 0, 0);
+    }
+  };
   float dw[V][8] = {};
+  if (kAhead) load(row);
   for (int it = 0; row < a.M; row += rows_step, it ^= 1) {
     const int64_t base = row * a.nvec;
     const float r = __ldg(a.rstd + row);
     uint4 gv[V], hv[V], dv[V];
+    if (!kAhead) load(row);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
+      gv[i] = gn[i];
+      hv[i] = hn[i];
       const int vec = tid + i * step;
-      const bool in = vec < a.nvec;
-      gv[i] = in ? __ldg(a.dy + base + vec) : make_uint4(0, 0, 0, 0);
-      hv[i] = in ? __ldg(a.h + base + vec) : make_uint4(0, 0, 0, 0);
-      dv[i] = in && a.dh ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
+      dv[i] = a.dh && vec < a.nvec ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
     }
+    if (kAhead) load(row + rows_step);
     float c = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -272,6 +286,7 @@ __global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
 __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, int n, int K, int w32,
                                                            void* dw) {
   __shared__ float sh[32][33];
+  cudaGridDependencySynchronize();
   const int k = blockIdx.x * 32 + (threadIdx.x & 31), rl = threadIdx.x >> 5;
   float s = 0.0f;
   if (k < K)
@@ -291,16 +306,14 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
 // Threads of a CTA that takes a row with two vectors a thread.
 int row_threads(int nvec, int v) { return ((nvec + v - 1) / v + 31) / 32 * 32; }
 
-// CTAs of the backward (also the rows of its workspace): two full SMs' worth
-// of threads each, no more than there are rows.
+// CTAs of the backward (also the rows of its workspace): as many as run at
+// once, no more than there are rows.
 int bwd_ctas(int64_t M, int nvec, int num_sms) {
-  if (nvec <= 128) {
-    const int64_t need = (M + WARP_ROWS - 1) / WARP_ROWS;
-    return static_cast<int>(need < 4 * num_sms ? need : 4 * num_sms);
-  }
-  const int per = 1024 / row_threads(nvec, 2) > 0 ? 1024 / row_threads(nvec, 2) : 1;
-  const int64_t most = static_cast<int64_t>(per) * num_sms;
-  return static_cast<int>(M < most ? M : most);
+  const int t = row_threads(nvec, 2);
+  const int per_sm = nvec <= 128 ? 4 : t <= 256 ? 768 / t : 1;
+  const int64_t need = nvec <= 128 ? (M + WARP_ROWS - 1) / WARP_ROWS : M;
+  const int64_t most = static_cast<int64_t>(per_sm) * num_sms;
+  return static_cast<int>(need < most ? need : most);
 }
 
 }  // namespace rms
@@ -345,22 +358,44 @@ int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const 
                            const float* rstd, int64_t M, int64_t K, void* dx, void* dw, void* ws,
                            cudaStream_t st, int num_sms, const char** why) {
   using namespace gl::rms;
-  BwdArgs a{static_cast<const uint4*>(dy), static_cast<const uint4*>(dh), static_cast<const uint4*>(h),
-            weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, static_cast<int>(K / 8),
-            w32, 1.0f / static_cast<float>(K)};
-  const int n = a.nvec, ctas = bwd_ctas(M, n, num_sms);
+  const int n = static_cast<int>(K / 8), t = row_threads(n, 2);
+  const int ctas = bwd_ctas(M, n, num_sms);
+  const BwdArgs a{static_cast<const uint4*>(dy), static_cast<const uint4*>(dh), static_cast<const uint4*>(h),
+                  weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, n, w32,
+                  1.0f / static_cast<float>(K)};
   if (ctas > 0) {  // no rows: dw is a sum over nothing
+    constexpr int W = 32 * WARP_ROWS;
     if (n <= 32)
-      rms_norm_bwd_kernel<1, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+      rms_norm_bwd_kernel<1, true, W, 4><<<ctas, W, 0, st>>>(a);
     else if (n <= 64)
-      rms_norm_bwd_kernel<2, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+      rms_norm_bwd_kernel<2, true, W, 3><<<ctas, W, 0, st>>>(a);
     else if (n <= 128)
-      rms_norm_bwd_kernel<4, true><<<ctas, 32 * WARP_ROWS, 0, st>>>(a);
+      rms_norm_bwd_kernel<4, true, W, 1><<<ctas, W, 0, st>>>(a);
+    else if (t <= 256)
+      rms_norm_bwd_kernel<2, false, 256, 3><<<ctas, t, 0, st>>>(a);
+    else if (t <= 512)
+      rms_norm_bwd_kernel<2, false, 512, 1><<<ctas, t, 0, st>>>(a);
     else
-      rms_norm_bwd_kernel<2, false><<<ctas, row_threads(n, 2), 0, st>>>(a);
-    if (const int rc = launched(why)) return rc;
+      rms_norm_bwd_kernel<2, false, 1024, 1><<<ctas, t, 0, st>>>(a);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+      *why = cudaGetErrorString(e);
+      return -2;
+    }
   }
-  rms_norm_dw_kernel<<<static_cast<unsigned>((K + 31) / 32), 1024, 0, st>>>(
-      static_cast<const float*>(ws), ctas, static_cast<int>(K), w32, dw);
-  return launched(why);
+  // launched while the first runs out; it waits for it on the device
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((K + 31) / 32));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = ctas > 0 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, rms_norm_dw_kernel, static_cast<const float*>(ws), ctas,
+                                           static_cast<int>(K), w32, dw);
+  if (e == cudaSuccess) return 0;
+  *why = cudaGetErrorString(e);
+  return -2;
 }
