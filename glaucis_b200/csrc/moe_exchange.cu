@@ -11,7 +11,9 @@
 // All are bound by HBM: every row is moved once, in 16-byte vectors.  Dispatch
 // goes by tokens, not by output rows, so a token is read once and stored k
 // times; a warp takes a 2 KB piece of a row, which gives even small calls
-// enough warps to reach all SMs.
+// enough warps to reach all SMs (pieces of 1 KB: 5 % slower).  It writes up to
+// nine tenths of what it moves: 4096 tokens, topk 8, rows of 7168 bytes take 58
+// us, 4.2 TB/s of stores, where a fill runs at 3.9 TB/s.
 #include "common.cuh"
 
 namespace gl {
@@ -164,12 +166,13 @@ struct CombineArgs {
   int* err;
 };
 
-// B choices of a token are loaded at a time, U vectors of a lane from each:
-// B U = 8 loads in flight a lane (4 of twice the size for fp32), which is what
-// reaches HBM's rate; a batch wider than topk would leave half of them empty
-// (16387 tokens, topk 2, K 4096: 132 us with B = 4, U = 2).
+// B choices of a token are loaded at a time, U vectors of a lane from each.  Four
+// loads in flight a lane with four CTAs an SM reach HBM's rate: 4096 tokens,
+// topk 8, K 7168 take 91 us with B = U = 2 (floor 90), 133 us with eight loads
+// and the two CTAs that their registers leave, 95 us with B = 4, U = 1; topk 2
+// 81, 92 and 81 us (16387 tokens, K 4096).
 template <bool kF32, int B, int U>
-__global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(256, 4) combine_kernel(const CombineArgs a) {
   const int lane = threadIdx.x & 31;
   const int segs = (a.nvec + 32 * U - 1) / (32 * U);
   const int64_t units = a.T * segs, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
@@ -237,9 +240,11 @@ struct CombineBwdArgs {
 };
 
 // A CTA takes a token: its gradient stays in registers (V vectors a thread)
-// while the rows of its choices pass.
+// while the rows of its choices pass.  Four CTAs an SM where the registers do
+// (4096 tokens, topk 8, K 7168: 167 us against 181 with two; 1.0 GB moved, half
+// of it written).
 template <int V, bool kF32>
-__global__ void __launch_bounds__(256) combine_bwd_kernel(const CombineBwdArgs a) {
+__global__ void __launch_bounds__(256, V <= 4 ? 4 : 2) combine_bwd_kernel(const CombineBwdArgs a) {
   __shared__ float part[MAX_K][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
@@ -354,11 +359,9 @@ int gl_launch_moe_combine(const void* y, int y_f32, const int32_t* pos, const fl
   const CombineArgs a{y, pos, weights, static_cast<const uint4*>(residual), T, rows, static_cast<int>(k),
                       static_cast<int>(K / 8), static_cast<uint4*>(out), err};
   if (k == 1)
-    y_f32 ? combine<true, 1, 4>(a, num_sms, st) : combine<false, 1, 8>(a, num_sms, st);
-  else if (k == 2)
-    y_f32 ? combine<true, 2, 2>(a, num_sms, st) : combine<false, 2, 4>(a, num_sms, st);
+    y_f32 ? combine<true, 1, 4>(a, num_sms, st) : combine<false, 1, 4>(a, num_sms, st);
   else
-    y_f32 ? combine<true, 4, 1>(a, num_sms, st) : combine<false, 4, 2>(a, num_sms, st);
+    y_f32 ? combine<true, 2, 2>(a, num_sms, st) : combine<false, 2, 2>(a, num_sms, st);
   return launched(why);
 }
 

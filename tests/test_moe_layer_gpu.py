@@ -1,0 +1,221 @@
+"""The operators around the experts' products run together, as a layer uses them:
+norm, router, rows into expert order, products, weighted sum onto the residual;
+for a prompt in e4m3, for generated tokens with 4-bit weights inside a CUDA
+graph, and for training through autograd."""
+import pytest
+import torch
+
+from glaucis_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F64 = torch.bfloat16, torch.float64
+
+
+def _rand(cuda, *shape, seed=0, scale=1.0, dtype=BF16):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=cuda) * scale).to(dtype)
+
+
+def _experts64(rows, sizes, weight):
+    """rows (fp64, expert order) times each expert's fp64 weight; zeros past the last group."""
+    out = torch.zeros((rows.shape[0], weight(0).shape[1]), dtype=F64, device=rows.device)
+    at = 0
+    for g, n in enumerate(sizes):
+        if n:
+            out[at:at + n] = rows[at:at + n] @ weight(g)
+            at += n
+    return out
+
+
+@pytest.mark.parametrize("T,E,k,K,N,pad", [(300, 16, 4, 1024, 512, 0), (129, 8, 2, 512, 256, 40), (1, 8, 2, 256, 128, 0)])
+def test_prompt_in_e4m3(cuda, T, E, k, K, N, pad):
+    x, res = _rand(cuda, T, K, seed=1), _rand(cuda, T, K, seed=2)
+    w = (1 + 0.1 * _rand(cuda, K, seed=3, dtype=torch.float32))
+    wg, rhs = _rand(cuda, K, E, seed=4, scale=0.05, dtype=torch.float32), _rand(cuda, E, K, N, seed=5, scale=0.02)
+    down = _rand(cuda, E, N, K, seed=6, scale=0.02)
+    mask = torch.arange(T, device=cuda) < T - pad if pad else None
+    f = ops.rms_norm_fwd(x, w, residual=res, output_quant=True)
+    r = ops.moe_route_fwd(f.y.float() @ wg, k, mask=mask)
+    a_q, a_s = ops.moe_dispatch_quant(f.q, f.s, r.pos, r.counts)
+    up = ops.gmm_fp8_fwd(a_q, a_s, *ops.quant_w_128x128(rhs), r.counts, out_dtype=BF16)
+    rows = int(r.counts.sum())
+    up[rows:] = 0
+    mid_q, mid_s = ops.quant_act_1x128(torch.nn.functional.silu(up))
+    y = ops.gmm_fp8_fwd(mid_q, mid_s, *ops.quant_w_128x128(down), r.counts, out_dtype=BF16)
+    y[rows:] = float("nan")  # rows of no group are not read
+    out = ops.moe_combine(y, r.pos, r.weights, r.counts, residual=f.h)
+    assert ops.device_status() == 0 and torch.isfinite(out).all()
+    assert rows == (T - pad) * k
+    if pad:
+        assert torch.equal(out[T - pad:], f.h[T - pad:])
+
+    # the same products on the same quantised operands in 64 bits
+    def deq(q, s):
+        return q.to(F64) * s.to(F64).repeat_interleave(128, -1)
+
+    def weights(t):
+        q, s = ops.quant_w_128x128(t)
+        return lambda g: q[g].to(F64) * s[g].to(F64).repeat_interleave(128, 0).repeat_interleave(128, 1)
+
+    sizes = r.counts.tolist()
+    # a product of e4m3 blocks: fp32 sums of 128 terms, then of K / 128 blocks; bf16 out
+    ref_up = _experts64(deq(a_q, a_s), sizes, weights(rhs))
+    mag = _experts64(deq(a_q, a_s).abs(), sizes, lambda g: weights(rhs)(g).abs())
+    assert ((up.to(F64) - ref_up).abs() <= 2.0 ** -8 * ref_up.abs() + 2.0 ** -13 * mag).all()
+    ref_y = _experts64(deq(mid_q, mid_s), sizes, weights(down))
+    mag = _experts64(deq(mid_q, mid_s).abs(), sizes, lambda g: weights(down)(g).abs())
+    assert ((y[:rows].to(F64) - ref_y[:rows]).abs() <= 2.0 ** -8 * ref_y[:rows].abs() + 2.0 ** -13 * mag[:rows]).all()
+    at = r.pos.clamp_min(0).long()
+    part = torch.where((r.pos >= 0)[:, :, None], y.to(F64)[at] * r.weights.to(F64)[:, :, None], 0)
+    ref = f.h.to(F64) + part.sum(1)
+    mag = f.h.to(F64).abs() + part.abs().sum(1)
+    assert ((out.to(F64) - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -20 * mag).all()
+
+
+def test_rows_are_quantised_once_or_per_choice_alike(cuda):
+    T, E, k, K = 200, 16, 4, 512
+    x, w = _rand(cuda, T, K), torch.ones(K, dtype=BF16, device=cuda)
+    f = ops.rms_norm_fwd(x, w, output_quant=True)
+    r = ops.moe_route_fwd(_rand(cuda, T, E, seed=1, dtype=torch.float32), k)
+    a_q, a_s = ops.moe_dispatch_quant(*ops.quant_act_1x128(f.y), r.pos, r.counts)
+    b_q, b_s = ops.quant_act_1x128(ops.moe_dispatch(f.y, r.pos, r.counts))
+    assert torch.equal(a_q.view(torch.uint8), b_q.view(torch.uint8)) and torch.equal(a_s, b_s)
+
+
+def test_generated_tokens_in_a_graph(cuda):
+    T, E, k, K, N = 3, 32, 4, 1024, 512
+    w = torch.ones(K, dtype=BF16, device=cuda)
+    wg = _rand(cuda, K, E, seed=1, scale=0.05, dtype=torch.float32)
+    up, down = (ops.quant_w4_128x1(_rand(cuda, E, a, b, seed=s, scale=0.02)) for a, b, s in ((K, N, 2), (N, K, 3)))
+
+    def layer(x, res):
+        f = ops.rms_norm_fwd(x, w, residual=res)
+        r = ops.moe_route(f.y.float() @ wg, k)
+        xs = ops.moe_dispatch(f.y, r.pos, r.counts)
+        mid = torch.nn.functional.silu(ops.gmm_w4_fwd(xs, *up, r.counts, out_dtype=BF16))
+        y = ops.gmm_w4_fwd(mid, *down, r.counts)
+        return ops.moe_combine(y, r.pos, r.weights, r.counts, residual=f.h)
+
+    x, res = _rand(cuda, T, K, seed=4), _rand(cuda, T, K, seed=5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x, res)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(x, res)
+    for seed in range(6, 12):
+        x.copy_(_rand(cuda, T, K, seed=seed))
+        res.copy_(_rand(cuda, T, K, seed=seed + 100))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ops.device_status() == 0
+        assert torch.equal(out, layer(x, res))
+
+
+def _train_inputs(cuda, T, E, K, N):
+    p = dict(x=_rand(cuda, T, K, seed=1), res=_rand(cuda, T, K, seed=2),
+             w=1 + 0.1 * _rand(cuda, K, seed=3, dtype=torch.float32),
+             wg=_rand(cuda, K, E, seed=4, scale=0.05, dtype=torch.float32), rhs=_rand(cuda, E, K, N, seed=5, scale=0.02))
+    return p, _rand(cuda, T, N, seed=6, scale=0.1)
+
+
+def _train_forward(p, k, mask, rows):
+    y, h = ops.rms_norm(p["x"], p["w"], residual=p["res"])
+    logits = y.float() @ p["wg"]
+    r = ops.moe_route(logits, k, mask=mask)
+    xs = ops.moe_dispatch(y, r.pos, r.counts, rows)
+    e = ops.gmm_fp8_blockwise(xs, p["rhs"], r.counts, out_dtype=BF16)
+    return y, h, logits, r, xs, e, ops.moe_combine(e, r.pos, r.weights, r.counts, residual=h)
+
+
+@pytest.mark.parametrize("T,E,k,K,pad", [(192, 8, 2, 512, 0), (256, 16, 4, 256, 50)])
+def test_training_step(cuda, T, E, k, K, pad):
+    """Autograd through the layer gives bit for bit what the operators' own
+    backward calls give, chained by hand (each of which its own tests hold to
+    the formulas and to differences)."""
+    p, dout = _train_inputs(cuda, T, E, K, K)
+    leaves = {n: t.clone().requires_grad_() for n, t in p.items()}
+    mask = torch.arange(T, device=cuda) < T - pad if pad else None
+    rows = (T * k + 127) // 128 * 128
+    y, h, logits, r, xs, e, out = _train_forward(leaves, k, mask, rows)
+    loss = (out.float() * dout.float()).sum() + 0.01 * r.balance_loss
+    got = dict(zip(leaves, torch.autograd.grad(loss, list(leaves.values()))))
+
+    with torch.no_grad():
+        f = ops.rms_norm_fwd(p["x"], p["w"], residual=p["res"])
+        rt = ops.moe_route_fwd(f.y.float() @ p["wg"], k, mask=mask)
+        assert torch.equal(f.y, y) and torch.equal(f.h, h) and torch.equal(rt.pos, r.pos)
+        de, dweights = ops.moe_combine_bwd(dout, e.detach(), rt.pos, rt.weights, rt.counts)
+        dxs, drhs = ops.gmm_fp8_blockwise_bwd(xs.detach(), p["rhs"], rt.counts, de)
+        dlogits = ops.moe_route_bwd(logits.detach(), rt, dweights, torch.tensor(0.01, device=cuda))
+        dy = ops.moe_dispatch_bwd(dxs, rt.pos) + (dlogits @ p["wg"].t()).to(BF16)
+        dx, dw = ops.rms_norm_bwd(dy, f.h, p["w"], f.rstd, dh=dout)
+        dwg = f.y.float().t() @ dlogits
+    assert torch.equal(got["rhs"], drhs) and torch.equal(got["wg"], dwg)
+    assert torch.equal(got["x"], dx) and torch.equal(got["res"], dx) and torch.equal(got["w"], dw)
+    if pad:  # padding reaches neither the router nor the experts: its gradient is the residual's
+        assert (dlogits[T - pad:] == 0).all()
+        assert torch.equal(dy[T - pad:], torch.zeros_like(dy[T - pad:]))
+    assert ops.device_status() == 0
+
+
+def test_training_step_in_a_graph(cuda):
+    """Forward and backward captured together replay to the eager gradients."""
+    T, E, k, K = 128, 8, 2, 256
+    p, dout = _train_inputs(cuda, T, E, K, K)
+    leaves = {n: t.clone().requires_grad_() for n, t in p.items()}
+
+    def step():
+        r, out = _train_forward(leaves, k, None, T * k)[3::3]
+        return torch.autograd.grad((out.float() * dout.float()).sum() + 0.01 * r.balance_loss, list(leaves.values()))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (20, 21):
+        with torch.no_grad():
+            leaves["x"].copy_(_rand(cuda, T, K, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [g.clone() for g in got]
+        for a, b in zip(replayed, step()):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_many_streams(cuda):
+    """The same calls under way on several streams at once give what they give alone."""
+    T, E, k, K = 500, 64, 6, 512
+    w = torch.ones(K, dtype=BF16, device=cuda)
+    xs = [_rand(cuda, T, K, seed=i) for i in range(4)]
+    zs = [_rand(cuda, T, E, seed=10 + i, dtype=torch.float32) for i in range(4)]
+    w4 = ops.quant_w4_128x1(_rand(cuda, E, K, 128, seed=30, scale=0.02))
+
+    def chain(x, z):
+        f = ops.rms_norm_fwd(x, w)
+        dx, dw = ops.rms_norm_bwd(x, f.h, w, f.rstd)
+        r = ops.moe_route_fwd(z, k)
+        rows = ops.moe_dispatch(f.y, r.pos, r.counts)
+        y = ops.gmm_w4_fwd(rows, *w4, r.counts, out_dtype=BF16)
+        return dx, dw, r.pos, r.balance_loss, ops.moe_combine(y, r.pos, r.weights, r.counts)
+
+    want = [chain(x, z) for x, z in zip(xs, zs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[] for _ in xs]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(chain(xs[i], zs[i]))
+    torch.cuda.synchronize()
+    for i in range(4):
+        for res in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
+    assert ops.device_status() == 0
