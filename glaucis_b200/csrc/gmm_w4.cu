@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
       }
     } else if (tiles < 0) {
       if (blockIdx.x == 0 && lane == 0) atomicExch(a.err, GL_DEV_BAD_GROUPS);
-    } else if (a.zero_tail) {
+    } else if (a.zero_tail && warp == WARPS + 1) {
       const int64_t words = a.N * (a.out_f32 ? 4 : 2) / 16;
       for (int64_t i = total * words + static_cast<int64_t>(blockIdx.x) * 32 + lane; i < a.M * words;
            i += static_cast<int64_t>(gridDim.x) * 32)

@@ -3,6 +3,8 @@ op launches on the current stream and never falls back to another backend.
 
 Op names and argument meaning mirror the Glaucis kernel templates
 (KE/examples/kernels/gmm_fp8_blockwise.py, KE/examples/kernels/chunk_gla.py).
+The operators around the grouped matmul (rms_norm*, moe_*, gmm_w4_fwd) have no
+counterpart there.
 """
 from __future__ import annotations
 
@@ -10,6 +12,7 @@ import contextlib
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -634,20 +637,23 @@ _NO_GUARD = contextlib.nullcontext()
 def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
     """Checks that every tensor is a contiguous one on `first`'s CUDA device;
     returns a context in which that device is the current one."""
-    dev = first.get_device() if first.is_cuda else -1
-    for t in (first, *rest):
-        if t is None:
-            continue
-        if not t.is_cuda or not t.is_contiguous():
+    dev = first.get_device()
+    if dev < 0 or not first.is_contiguous():
+        _need_cuda(first)
+    for t in rest:
+        if t is not None and (t.get_device() != dev or not t.is_contiguous()):
             _need_cuda(t)
-        if t.get_device() != dev:
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
     return _NO_GUARD if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _new(like: torch.Tensor, t: Optional[torch.Tensor], shape, dtype: torch.dtype, name: str) -> torch.Tensor:
-    """_out on `like`'s device."""
-    return like.new_empty(shape, dtype=dtype) if t is None else _out(t, shape, dtype, like.device, name)
+    """_out on `like`'s device (empty_like, the cheapest call, where it will do)."""
+    if t is not None:
+        return _out(t, shape, dtype, like.device, name)
+    if like.shape == shape:
+        return torch.empty_like(like) if like.dtype == dtype else torch.empty_like(like, dtype=dtype)
+    return torch.empty(*shape, dtype=dtype, device=like.device)
 
 
 class RMSNormForward(NamedTuple):
@@ -761,6 +767,7 @@ class _RMSNorm(torch.autograd.Function):
         return f.y if residual is None else (f.y, f.h)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         if dh is not None:
@@ -824,7 +831,7 @@ def moe_route_fwd(logits: torch.Tensor, topk: int, *, mask: Optional[torch.Tenso
     E <= 1024, topk <= 32."""
     with _same_device(logits, mask):
         T, E = _route_check(logits, mask)
-        ids = logits.new_empty((T, topk), dtype=torch.int32)
+        ids = torch.empty(T, topk, dtype=torch.int32, device=logits.device)
         pos = torch.empty_like(ids)
         weights = torch.empty_like(ids, dtype=torch.float32)
         counts = logits.new_empty(E, dtype=torch.int32)
@@ -875,6 +882,7 @@ class _MoERoute(torch.autograd.Function):
         return r.ids, r.weights, r.counts, r.pos, r.balance_loss, r.routed
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, _ids, dweights, _counts, _pos, dloss, _routed):
         if dweights is None and dloss is None:
             return None, None, None, None
@@ -962,7 +970,7 @@ def moe_dispatch_bwd(dout: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         T, _ = _pos_check(pos)
         if dout.dtype not in (torch.bfloat16, torch.float32) or dout.dim() != 2:
             raise ValueError("dout must be bf16 or fp32 [rows, K]")
-        dx = dout.new_empty((T, dout.shape[1]), dtype=torch.bfloat16)
+        dx = torch.empty(T, dout.shape[1], dtype=torch.bfloat16, device=dout.device)
         _combine(dout, pos, None, None, dx)
     return dx
 
@@ -974,6 +982,7 @@ class _MoEDispatch(torch.autograd.Function):
         return moe_dispatch_fwd(x, pos, group_sizes, rows)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         return moe_dispatch_bwd(dout.to(torch.bfloat16).contiguous(), ctx.saved_tensors[0]), None, None, None
 
@@ -981,9 +990,10 @@ class _MoEDispatch(torch.autograd.Function):
 def moe_dispatch(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
                  rows: Optional[int] = None) -> torch.Tensor:
     """Rows of the tokens in expert order: out[pos[t, j]] = x[t] (bf16 [T, K])
-    for the pos and counts of moe_route; the lhs of gmm_fp8_blockwise with
-    group_sizes = counts.  `rows` (default T * topk) is the number of output
-    rows; those past sum(group_sizes) are zero.  Differentiable in x (bf16)."""
+    for the pos and counts of moe_route (distinct rows below sum(group_sizes), a
+    negative one is skipped); the lhs of gmm_fp8_blockwise with group_sizes =
+    counts.  `rows` (default T * topk) is the number of output rows; those past
+    sum(group_sizes) are zero.  Differentiable in x (bf16)."""
     if torch.is_grad_enabled() and x.requires_grad:
         if x.dtype != torch.bfloat16:
             raise ValueError("the differentiable moe_dispatch takes bf16")
@@ -1041,6 +1051,7 @@ class _MoECombine(torch.autograd.Function):
         return moe_combine_fwd(y, pos, weights, residual=residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         y, pos, weights, group_sizes = ctx.saved_tensors
         dout = dout.to(torch.bfloat16).contiguous()
@@ -1107,7 +1118,7 @@ def gmm_w4_fwd(x: torch.Tensor, w4: torch.Tensor, s: torch.Tensor, group_sizes: 
             raise ValueError("out must be a contiguous bf16 or fp32 [M, N] tensor")
         flags = _lib.GL_W4_ZERO_TAIL if out is None else 0
         if out is None:
-            out = x.new_empty((M, N), dtype=out_dtype)
+            out = torch.empty(M, N, dtype=out_dtype, device=x.device)
         code = _lib.GL_OUT_F32 if out.dtype == torch.float32 else _lib.GL_OUT_BF16
         lib = _lib.load()
         ws_bytes = lib.gl_gmm_w4_workspace_bytes(M, K)

@@ -190,6 +190,15 @@ def test_training_step_in_a_graph(cuda):
             assert torch.equal(a, b)
 
 
+def test_second_derivatives_are_refused(cuda):
+    p, dout = _train_inputs(cuda, 128, 8, 256, 256)
+    x = p["x"].requires_grad_()
+    y = ops.rms_norm(x, p["w"])
+    g, = torch.autograd.grad(y, x, dout.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.float().sum(), dout)
+
+
 def test_calls_on_many_streams(cuda):
     """The same calls under way on several streams at once give what they give alone."""
     T, E, k, K = 500, 64, 6, 512
