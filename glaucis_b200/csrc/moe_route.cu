@@ -49,11 +49,19 @@ struct Args {
   int* live;            // [CTAs]        }
 };
 
+// Warps of a CTA of the second launch: more, where the first one's registers
+// and rows of sums are not in the way.
 template <int V>
+constexpr int rank_warps() {
+  return V <= 16 ? 32 : 16;
+}
+
+// W warps, P rows of sums.
+template <int V, int W, int P>
 struct Shared {
   union {
-    float psum[warps<V>()][32 * V];     // each warp's sum of the softmax
-    uint16_t cnt[warps<V>()][32 * V];   // choices of an expert in a batch of entries
+    float psum[P][32 * V];     // parts of the softmax's sum
+    uint16_t cnt[W][32 * V];   // choices of an expert in a batch of entries
   };
   int hist[32 * V];   // this CTA's counts, then the row of an expert's next choice
   int total[32 * V];
@@ -83,6 +91,11 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
+
+template <int V>
+using RouteShared = Shared<V, warps<V>(), warps<V>()>;  // a row of sums for every warp
+template <int V>
+using RankShared = Shared<V, rank_warps<V>(), (rank_warps<V>() > V ? rank_warps<V>() / V : 1)>;
 
 // The lane's V logits of token t (experts lane V .. lane V + V - 1), -inf past
 // the last expert and for a token that the mask takes out.
@@ -172,14 +185,18 @@ __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float 
 }
 
 // A lane's keys and where they are, so that the largest is at hand and the next
-// takes its place when it is chosen.  Up to four are kept sorted (equal keys in
-// the experts' order); of more, the largest is looked for again.
+// takes its place when it is chosen.  Fours of consecutive experts are kept
+// sorted (equal keys in the experts' order), and the largest is that of the
+// fours' heads; of 16 and more, for which registers run short, it is looked for
+// again.
 template <int V>
 struct Keys {
-  static constexpr bool kSorted = V <= 4;
+  static constexpr bool kSorted = V <= 8;
+  static constexpr int F = V < 4 ? V : 4, N = V / F;  // keys of a four, fours
   uint32_t key[V];
-  int at[V];  // kSorted: expert of each; else at[0]: index of the largest
+  int at[V];  // kSorted: index of each; else at[0]: index of the largest
   uint32_t own;
+  int four;   // whose head it is
 
   __device__ __forceinline__ void order(int i, int j) {  // i < j
     if (key[j] > key[i]) {
@@ -193,45 +210,62 @@ struct Keys {
   }
   __device__ __forceinline__ void look() {
     own = key[0];
-    at[0] = 0;
+    if constexpr (kSorted) {
+      four = 0;
 #pragma unroll
-    for (int i = 1; i < V; ++i)
-      if (key[i] > own) {
-        own = key[i];
-        at[0] = i;
-      }
+      for (int n = 1; n < N; ++n)
+        if (key[n * F] > own) {
+          own = key[n * F];
+          four = n;
+        }
+    } else {
+      at[0] = 0;
+#pragma unroll
+      for (int i = 1; i < V; ++i)
+        if (key[i] > own) {
+          own = key[i];
+          at[0] = i;
+        }
+    }
   }
   __device__ __forceinline__ void begin(const float (&z)[V]) {
-    const int e0 = (threadIdx.x & 31) * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
     if constexpr (kSorted) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) at[i] = e0 + i;
-      // insertion by neighbours only, which keeps equal keys in order
+      for (int i = 0; i < V; ++i) at[i] = i;
+      // exchange of neighbours only, which keeps equal keys in order
 #pragma unroll
-      for (int n = V - 1; n > 0; --n)
+      for (int b = 0; b < V; b += F)
 #pragma unroll
-        for (int i = 0; i < n; ++i) order(i, i + 1);
-      own = key[0];
-    } else {
-      look();
+        for (int n = F - 1; n > 0; --n)
+#pragma unroll
+          for (int i = 0; i < n; ++i) order(b + i, b + i + 1);
     }
+    look();
   }
   __device__ __forceinline__ int expert() const {
-    if constexpr (kSorted) return at[0];
-    return (threadIdx.x & 31) * V + at[0];
+    int i = at[0];
+    if constexpr (kSorted) {
+#pragma unroll
+      for (int n = 1; n < N; ++n) i = four == n ? at[n * F] : i;
+    }
+    return (threadIdx.x & 31) * V + i;
   }
   // Takes the largest away (in the lane with `won`).
   __device__ __forceinline__ void next(bool won) {
     if constexpr (kSorted) {
 #pragma unroll
-      for (int i = 0; i + 1 < V; ++i) {
-        key[i] = won ? key[i + 1] : key[i];
-        at[i] = won ? at[i + 1] : at[i];
+      for (int n = 0; n < N; ++n) {
+        const bool here = won && (N == 1 || four == n);
+#pragma unroll
+        for (int i = n * F; i + 1 < (n + 1) * F; ++i) {
+          key[i] = here ? key[i + 1] : key[i];
+          at[i] = here ? at[i + 1] : at[i];
+        }
+        key[(n + 1) * F - 1] = here ? 0 : key[(n + 1) * F - 1];
       }
-      key[V - 1] = won ? 0 : key[V - 1];
-      own = key[0];
+      look();
     } else if (won) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
@@ -244,7 +278,7 @@ struct Keys {
 // Routes tokens [t0, t1): ids, weights; counts into sh.hist, each warp's
 // softmax sums into sh.psum and the number of routed tokens into sh.live.
 template <int V>
-__device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& sh) {
+__device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, RouteShared<V>& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) sh.hist[e] = 0;
   if (threadIdx.x == 0) sh.live = 0;
@@ -300,8 +334,8 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, Shared<V>& s
 
 // Exclusive scan of sh.total over the experts, added to sh.hist: warp 0, V
 // consecutive experts a lane.
-template <int V>
-__device__ __forceinline__ void add_scan(Shared<V>& sh) {
+template <int V, class Sh>
+__device__ __forceinline__ void add_scan(Sh& sh) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int n[V], own = 0;
@@ -328,8 +362,8 @@ __device__ __forceinline__ void add_scan(Shared<V>& sh) {
 
 // sh.total: choices of every expert; sh.hist: the first row of this CTA's
 // choices of it.  `ctas` CTAs' counts, `cta` of them before this one.
-template <int V>
-__device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
+template <int V, class Sh>
+__device__ void first_rows(const Args& a, Sh& sh, int ctas, int cta) {
   for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) sh.total[e] = sh.hist[e] = 0;
   __syncthreads();
   const int slices = blockDim.x >= 32 * V ? blockDim.x / (32 * V) : 1;
@@ -337,7 +371,7 @@ __device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
     const int e = i % (32 * V);
     if (e >= a.E) continue;
     int before = 0, total = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int b = i / (32 * V); b < ctas; b += slices) {
       const int h = __ldcg(a.hist + static_cast<int64_t>(b) * a.E + e);
       total += h;
@@ -353,13 +387,13 @@ __device__ void first_rows(const Args& a, Shared<V>& sh, int ctas, int cta) {
 // Rows of the choices of tokens [t0, t1), a batch of one choice a thread at a
 // time: rank among the batch's earlier choices of the same expert (within the
 // warp by match, over the warps by a column of counts).
-template <int V>
-__device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1) {
+template <int V, class Sh>
+__device__ void assign_rows(const Args& a, Sh& sh, int64_t t0, int64_t t1) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n0 = t0 * a.k, n1 = t1 * a.k;
   for (int64_t b = n0; b < n1; b += blockDim.x) {
     const int64_t left = n1 - b;
-    const int used = left < blockDim.x ? static_cast<int>((left + 31) / 32) : warps<V>();
+    const int used = left < blockDim.x ? static_cast<int>((left + 31) / 32) : static_cast<int>(blockDim.x >> 5);
     uint32_t* zero = reinterpret_cast<uint32_t*>(&sh.cnt[0][0]);
     for (int i = threadIdx.x; i < used * 16 * V; i += blockDim.x) zero[i] = 0;
     const int64_t n = b + threadIdx.x;
@@ -388,8 +422,8 @@ __device__ void assign_rows(const Args& a, Shared<V>& sh, int64_t t0, int64_t t1
 
 // counts and the loss: sh.total are all choices of an expert, sh.psum[0..rows)
 // parts of the softmax's sum over `n` routed tokens.
-template <int V>
-__device__ void finish(const Args& a, Shared<V>& sh, int rows, int n) {
+template <int V, class Sh>
+__device__ void finish(const Args& a, Sh& sh, int rows, int n) {
   float part = 0.0f, chosen = 0.0f;
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     float p = 0.0f;
@@ -409,8 +443,8 @@ __device__ void finish(const Args& a, Shared<V>& sh, int rows, int n) {
   }
   __syncthreads();
   if (warp == 0) {
-    part = warp_sum(lane < warps<V>() ? sh.red[0][lane] : 0.0f);
-    chosen = warp_sum(lane < warps<V>() ? sh.red[1][lane] : 0.0f);
+    part = warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? sh.red[0][lane] : 0.0f);
+    chosen = warp_sum(lane < static_cast<int>(blockDim.x >> 5) ? sh.red[1][lane] : 0.0f);
     if (lane == 0) {
       const float tokens = static_cast<float>(max(n, 1));
       *a.loss = static_cast<float>(a.E) * (part / fmaxf(chosen, 1.0f) / tokens);
@@ -422,7 +456,7 @@ __device__ void finish(const Args& a, Shared<V>& sh, int rows, int n) {
 // One CTA takes every token.
 template <int V>
 __global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a) {
-  __shared__ Shared<V> sh;
+  __shared__ RouteShared<V> sh;
   route_tokens<V>(a, 0, a.T, sh);
   for (int e = threadIdx.x; e < 32 * V; e += blockDim.x) {
     sh.total[e] = sh.hist[e];
@@ -437,7 +471,7 @@ __global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a
 // First of two launches: the choices, and what the CTA adds to counts and loss.
 template <int V>
 __global__ void __launch_bounds__(32 * warps<V>()) route_kernel(const Args a) {
-  __shared__ Shared<V> sh;
+  __shared__ RouteShared<V> sh;
   cudaTriggerProgrammaticLaunchCompletion();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
   const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
@@ -454,8 +488,8 @@ __global__ void __launch_bounds__(32 * warps<V>()) route_kernel(const Args a) {
 
 // Second launch: the CTAs of the first rank their choices, one more finishes.
 template <int V>
-__global__ void __launch_bounds__(32 * warps<V>()) rank_kernel(const Args a) {
-  __shared__ Shared<V> sh;
+__global__ void __launch_bounds__(32 * rank_warps<V>()) rank_kernel(const Args a) {
+  __shared__ RankShared<V> sh;
   cudaGridDependencySynchronize();
   const int ctas = gridDim.x - 1, cta = blockIdx.x;
   first_rows<V>(a, sh, ctas, cta);
@@ -466,7 +500,7 @@ __global__ void __launch_bounds__(32 * warps<V>()) rank_kernel(const Args a) {
       const int e = i % (32 * V);
       float s = 0.0f;
       if (e < a.E) {
-#pragma unroll 8
+#pragma unroll 16
         for (int b = i / (32 * V); b < ctas; b += slices) s += __ldcg(a.psum + static_cast<int64_t>(b) * a.E + e);
       }
       sh.psum[i / (32 * V)][e] = s;
@@ -643,7 +677,7 @@ int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
       // launched while the first runs out; it waits for it on the device
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(ctas + 1);
-      cfg.blockDim = dim3(32 * warps<V>());
+      cfg.blockDim = dim3(32 * rank_warps<V>());
       cfg.stream = st;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

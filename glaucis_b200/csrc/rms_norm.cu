@@ -19,7 +19,7 @@ namespace gl {
 namespace rms {
 
 constexpr int MAX_K = 16384;  // 1024 threads x 2 vectors x 8 features
-constexpr int WARP_ROWS = 8;  // rows of a CTA when a warp takes a row
+constexpr int SMALL_T = 256;  // threads of a CTA whose warps take rows of their own
 
 struct FwdArgs {
   const uint4* x;
@@ -68,29 +68,36 @@ __device__ __forceinline__ void load_w8(const void* w, int w32, int vec, float (
   }
 }
 
-// Sum over the threads of a row: a warp's own when a warp takes a row, else
-// over the CTA's warps through `part` (one slot per warp).
-template <bool kWarpRow>
+// Sum over the threads of a row: L lanes of a warp, or (L = 0) the CTA's warps
+// through `part` (one slot per warp).
+template <int L>
 __device__ __forceinline__ float row_sum(float v, float* part) {
+  if (L == 16) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+  }
   v = warp_sum(v);
-  if (kWarpRow) return v;
+  if (L == 32) return v;
   const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   if (lane == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   return warp_sum(lane < nw ? part[lane] : 0.0f);
 }
 
-// V vectors a thread.  kWarpRow: a warp per row, WARP_ROWS rows a CTA; else a
-// CTA per row.
-template <int V, bool kWarpRow>
-__global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
-    rms_norm_fwd_kernel(const FwdArgs a) {
+// V vectors a thread.  L lanes a row (16 up to 128 features, a warp up to 1024),
+// SMALL_T threads a CTA; L = 0: a CTA per row.
+template <int V, int L>
+__global__ void __launch_bounds__(L ? SMALL_T : 1024) rms_norm_fwd_kernel(const FwdArgs a) {
+  constexpr int LL = L ? L : 1;
   __shared__ float part[32];
-  const int64_t row = kWarpRow ? static_cast<int64_t>(blockIdx.x) * WARP_ROWS + (threadIdx.x >> 5)
-                               : static_cast<int64_t>(blockIdx.x);
-  if (kWarpRow && row >= a.M) return;
-  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
-  const int step = kWarpRow ? 32 : blockDim.x;
+  const int64_t row = L ? static_cast<int64_t>(blockIdx.x) * (SMALL_T / LL) + threadIdx.x / LL
+                        : static_cast<int64_t>(blockIdx.x);
+  // rows end inside a warp (two a warp): past them a thread goes on with none
+  const bool live = !L || row < a.M;
+  const int tid = L ? threadIdx.x % LL : threadIdx.x;
+  const int step = L ? L : blockDim.x;
+  const int nvec = live ? a.nvec : 0;
   const int64_t base = row * a.nvec;
 
   // plain loads: h may be x's or the residual's own buffer (every element is
@@ -99,8 +106,8 @@ __global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int vec = tid + i * step;
-    xv[i] = vec < a.nvec ? a.x[base + vec] : make_uint4(0, 0, 0, 0);
-    if (a.res) rv[i] = vec < a.nvec ? a.res[base + vec] : make_uint4(0, 0, 0, 0);
+    xv[i] = vec < nvec ? a.x[base + vec] : make_uint4(0, 0, 0, 0);
+    if (a.res) rv[i] = vec < nvec ? a.res[base + vec] : make_uint4(0, 0, 0, 0);
   }
   float sum = 0.0f;
 #pragma unroll
@@ -114,21 +121,21 @@ __global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] += g[j];
       xv[i] = pack8(f);  // the sum as it is stored: the one rounding of h
-      if (vec < a.nvec) a.h[base + vec] = xv[i];
+      if (vec < nvec) a.h[base + vec] = xv[i];
       unpack8(xv[i], f);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
   }
-  sum = row_sum<kWarpRow>(sum, part);
+  sum = row_sum<L>(sum, part);
   const float r = rsqrtf(fmaf(sum, a.inv_k, a.eps));
-  if (a.rstd && tid == 0) a.rstd[row] = r;
+  if (a.rstd && tid == 0 && live) a.rstd[row] = r;
 
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int vec = tid + i * step;
     float f[8], w[8];
-    if (vec < a.nvec) {
+    if (vec < nvec) {
       unpack8(xv[i], f);
       load_w8(a.w, a.w32, vec, w);
 #pragma unroll
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(kWarpRow ? 32 * WARP_ROWS : 1024)
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
       const float s = m == 0.0f ? 1.0f : m / 448.0f;
-      if (vec < a.nvec) {
+      if (vec < nvec) {
         // one division per block; blocks whose reciprocal would overflow (or
         // whose maximum is infinite) divide each element
         if (s >= 0x1p-100f && s <= 3.40282347e38f) {
@@ -182,20 +189,20 @@ struct BwdArgs {
   float inv_k;
 };
 
-// A persistent CTA takes rows blockIdx.x, + gridDim.x, ... (kWarpRow: a warp
-// each) and keeps its columns' share of dw in registers.  dy and h of the next
+// A persistent CTA takes rows blockIdx.x, + gridDim.x, ... (L lanes each, or L =
+// 0: the CTA one row at a time) and keeps its columns' share of dw in registers.  dy and h of the next
 // row are loaded while this row's sum is under way (where MAX_T leaves the
 // registers), dh, which only dx needs, with the row itself.
-template <int V, bool kWarpRow, int MAX_T, int CTAS>
+template <int V, int L, int MAX_T, int CTAS>
 __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs a) {
   constexpr bool kAhead = MAX_T <= 512;
+  constexpr int LL = L ? L : 1, ROWS = L ? SMALL_T / LL : 1;
   __shared__ float part[2][32];
-  __shared__ float cross[kWarpRow ? WARP_ROWS : 1][kWarpRow ? 32 * V * 8 : 1];
-  const int tid = kWarpRow ? threadIdx.x & 31 : threadIdx.x;
-  const int step = kWarpRow ? 32 : blockDim.x;
-  const int64_t rows_step = kWarpRow ? static_cast<int64_t>(gridDim.x) * WARP_ROWS : gridDim.x;
-  int64_t row = kWarpRow ? static_cast<int64_t>(blockIdx.x) * WARP_ROWS + (threadIdx.x >> 5)
-                         : static_cast<int64_t>(blockIdx.x);
+  __shared__ float cross[ROWS][L ? L * V * 8 : 1];
+  const int tid = L ? threadIdx.x % LL : threadIdx.x;
+  const int step = L ? L : blockDim.x;
+  const int64_t rows_step = static_cast<int64_t>(gridDim.x) * ROWS;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + (L ? threadIdx.x / LL : 0);
   uint4 gn[V], hn[V];
   auto load = [&](int64_t r) {
 #pragma unroll
@@ -208,9 +215,13 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
   };
   float dw[V][8] = {};
   if (kAhead) load(row);
-  for (int it = 0; row < a.M; row += rows_step, it ^= 1) {
+  // as many rounds for every lane of a warp (rows may end inside one)
+  const int64_t rounds = (a.M - static_cast<int64_t>(blockIdx.x) * ROWS + rows_step - 1) / rows_step;
+  for (int64_t n = 0; n < rounds; ++n, row += rows_step) {
+    const int it = static_cast<int>(n & 1);
     const int64_t base = row * a.nvec;
-    const float r = __ldg(a.rstd + row);
+    const int nvec = row < a.M ? a.nvec : 0;
+    const float r = row < a.M ? __ldg(a.rstd + row) : 0.0f;
     uint4 gv[V], hv[V], dv[V];
     if (!kAhead) load(row);
 #pragma unroll
@@ -218,14 +229,14 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
       gv[i] = gn[i];
       hv[i] = hn[i];
       const int vec = tid + i * step;
-      dv[i] = a.dh && vec < a.nvec ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
+      dv[i] = a.dh && vec < nvec ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
     }
     if (kAhead) load(row + rows_step);
     float c = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int vec = tid + i * step;
-      if (vec < a.nvec) {
+      if (vec < nvec) {
         float g[8], h[8], w[8];
         unpack8(gv[i], g);
         unpack8(hv[i], h);
@@ -240,11 +251,11 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
     }
     // two sets of slots: a warp may reach the next row's sum while another
     // still reads this one's
-    c = row_sum<kWarpRow>(c, part[it]) * a.inv_k;
+    c = row_sum<L>(c, part[it]) * a.inv_k;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int vec = tid + i * step;
-      if (vec < a.nvec) {
+      if (vec < nvec) {
         float g[8], h[8], d[8], w[8];
         unpack8(gv[i], g);
         unpack8(hv[i], h);
@@ -257,16 +268,16 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
     }
   }
   float* out = a.part + static_cast<int64_t>(blockIdx.x) * a.nvec * 8;
-  if (kWarpRow) {
+  if (L) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cross[threadIdx.x >> 5][(tid + i * 32) * 8 + j] = dw[i][j];
+      for (int j = 0; j < 8; ++j) cross[threadIdx.x / LL][(tid + i * L) * 8 + j] = dw[i][j];
     __syncthreads();
     for (int k = threadIdx.x; k < a.nvec * 8; k += blockDim.x) {
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < WARP_ROWS; ++i) s += cross[i][k];
+      for (int i = 0; i < ROWS; ++i) s += cross[i][k];
       out[k] = s;
     }
   } else {
@@ -306,13 +317,24 @@ __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, in
 // Threads of a CTA that takes a row with two vectors a thread.
 int row_threads(int nvec, int v) { return ((nvec + v - 1) / v + 31) / 32 * 32; }
 
-// CTAs of the backward (also the rows of its workspace): as many as run at
-// once, no more than there are rows.
-int bwd_ctas(int64_t M, int nvec, int num_sms) {
+// The backward's variant for a row length: as many CTAs of it as run at once on
+// an SM (also given to the compiler), and the rows that a CTA takes at a time.
+struct BwdShape {
+  int threads, rows, per_sm;
+};
+
+BwdShape bwd_shape(int nvec) {
+  if (nvec <= 16) return {SMALL_T, SMALL_T / 16, 4};
+  if (nvec <= 32) return {SMALL_T, SMALL_T / 32, 4};
+  if (nvec <= 64) return {SMALL_T, SMALL_T / 32, 3};
   const int t = row_threads(nvec, 2);
-  const int per_sm = nvec <= 128 ? 4 : t <= 256 ? 768 / t : 1;
-  const int64_t need = nvec <= 128 ? (M + WARP_ROWS - 1) / WARP_ROWS : M;
-  const int64_t most = static_cast<int64_t>(per_sm) * num_sms;
+  return {t, 1, t <= 256 ? 768 / t : t <= 384 ? 2 : 1};
+}
+
+// CTAs of the backward (also the rows of its workspace).
+int bwd_ctas(int64_t M, int nvec, int num_sms) {
+  const BwdShape b = bwd_shape(nvec);
+  const int64_t need = (M + b.rows - 1) / b.rows, most = static_cast<int64_t>(b.per_sm) * num_sms;
   return static_cast<int>(need < most ? need : most);
 }
 
@@ -335,18 +357,19 @@ int gl_launch_rms_norm_fwd(const void* x, const void* residual, const void* weig
             static_cast<uint4*>(h), static_cast<uint4*>(y), static_cast<uint2*>(q), s, rstd, M,
             static_cast<int>(K / 8), w32, 1.0f / static_cast<float>(K), eps};
   const int n = a.nvec;
-  if (n <= 128) {
-    const unsigned ctas = static_cast<unsigned>((M + WARP_ROWS - 1) / WARP_ROWS);
-    const int t = 32 * WARP_ROWS;
-    if (n <= 32)
-      rms_norm_fwd_kernel<1, true><<<ctas, t, 0, st>>>(a);
-    else if (n <= 64)
-      rms_norm_fwd_kernel<2, true><<<ctas, t, 0, st>>>(a);
-    else
-      rms_norm_fwd_kernel<4, true><<<ctas, t, 0, st>>>(a);
-  } else {
-    rms_norm_fwd_kernel<2, false><<<static_cast<unsigned>(M), row_threads(n, 2), 0, st>>>(a);
-  }
+  const auto ctas = [&](int lanes) { return static_cast<unsigned>((M + SMALL_T / lanes - 1) / (SMALL_T / lanes)); };
+  if (n <= 16)
+    rms_norm_fwd_kernel<1, 16><<<ctas(16), SMALL_T, 0, st>>>(a);
+  else if (n <= 32)
+    rms_norm_fwd_kernel<1, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 64)
+    rms_norm_fwd_kernel<2, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 128)
+    rms_norm_fwd_kernel<4, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 1024)
+    rms_norm_fwd_kernel<2, 0><<<static_cast<unsigned>(M), row_threads(n, 2), 0, st>>>(a);
+  else  // two CTAs of half the threads an SM more: K = 12288 in bf16 59 -> 47 us (5461 rows)
+    rms_norm_fwd_kernel<4, 0><<<static_cast<unsigned>(M), row_threads(n, 4), 0, st>>>(a);
   return launched(why);
 }
 
@@ -364,19 +387,20 @@ int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const 
                   weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, n, w32,
                   1.0f / static_cast<float>(K)};
   if (ctas > 0) {  // no rows: dw is a sum over nothing
-    constexpr int W = 32 * WARP_ROWS;
-    if (n <= 32)
-      rms_norm_bwd_kernel<1, true, W, 4><<<ctas, W, 0, st>>>(a);
+    if (n <= 16)
+      rms_norm_bwd_kernel<1, 16, SMALL_T, 4><<<ctas, SMALL_T, 0, st>>>(a);
+    else if (n <= 32)
+      rms_norm_bwd_kernel<1, 32, SMALL_T, 4><<<ctas, SMALL_T, 0, st>>>(a);
     else if (n <= 64)
-      rms_norm_bwd_kernel<2, true, W, 3><<<ctas, W, 0, st>>>(a);
-    else if (n <= 128)
-      rms_norm_bwd_kernel<4, true, W, 1><<<ctas, W, 0, st>>>(a);
+      rms_norm_bwd_kernel<2, 32, SMALL_T, 3><<<ctas, SMALL_T, 0, st>>>(a);
     else if (t <= 256)
-      rms_norm_bwd_kernel<2, false, 256, 3><<<ctas, t, 0, st>>>(a);
+      rms_norm_bwd_kernel<2, 0, 256, 3><<<ctas, t, 0, st>>>(a);
+    else if (t <= 384)
+      rms_norm_bwd_kernel<2, 0, 384, 2><<<ctas, t, 0, st>>>(a);
     else if (t <= 512)
-      rms_norm_bwd_kernel<2, false, 512, 1><<<ctas, t, 0, st>>>(a);
+      rms_norm_bwd_kernel<2, 0, 512, 1><<<ctas, t, 0, st>>>(a);
     else
-      rms_norm_bwd_kernel<2, false, 1024, 1><<<ctas, t, 0, st>>>(a);
+      rms_norm_bwd_kernel<2, 0, 1024, 1><<<ctas, t, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
       *why = cudaGetErrorString(e);
