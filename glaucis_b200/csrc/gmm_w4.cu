@@ -618,6 +618,8 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
     const int4 pj = ct.part[l];
     if (pj.y <= 2)
       add_parts<1, 12>(a, pj, from, to, from_last);
+    else if (pj.y <= 4)
+      add_parts<2, 6>(a, pj, from, to, from_last);
     else
       add_parts<4, 3>(a, pj, from, to, from_last);
   }

@@ -169,16 +169,22 @@ __device__ __forceinline__ bool takes_part(const float (&z)[V]) {
 }
 
 // e^x for x <= 0 as 2^(x log2 e): two roundings of the exponent, |x| 2^-24
-// relative each, where subtracting the row's maximum already made one.
-__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.44269504f); }
+// relative each, where subtracting the row's maximum already made one.  Results
+// below 2^-126 of the largest numerator are 0.
+__device__ __forceinline__ float exp_of(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+  return r;
+}
 
-// Softmax numerators e of the logits z; returns 1 / their sum.
+// Softmax numerators e of the logits z (0 where z is -inf and zmax is not);
+// returns 1 / their sum.
 template <int V>
 __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float (&e)[V]) {
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    e[i] = z[i] == -INFINITY ? 0.0f : exp_of(z[i] - zmax);
+    e[i] = exp_of(z[i] - zmax);
     s += e[i];
   }
   return __fdividef(1.0f, warp_sum(s));  // the sum is 1 to 1024: within 2 ulp
@@ -257,13 +263,14 @@ struct Keys {
     if constexpr (kSorted) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const bool here = won && (N == 1 || four == n);
+        if (won && (N == 1 || four == n)) {
 #pragma unroll
-        for (int i = n * F; i + 1 < (n + 1) * F; ++i) {
-          key[i] = here ? key[i + 1] : key[i];
-          at[i] = here ? at[i + 1] : at[i];
+          for (int i = n * F; i + 1 < (n + 1) * F; ++i) {
+            key[i] = key[i + 1];
+            at[i] = at[i + 1];
+          }
+          key[(n + 1) * F - 1] = 0;
         }
-        key[(n + 1) * F - 1] = here ? 0 : key[(n + 1) * F - 1];
       }
       look();
     } else if (won) {
@@ -293,11 +300,11 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, RouteShared<
     if (t + warps<V>() < t1) load_token<V>(a, t + warps<V>(), next);
     int id = -1;
     float p = 0.0f;
-    if (takes_part<V>(z)) {
+    Keys<V> keys;
+    keys.begin(z);
+    uint32_t m = __reduce_max_sync(FULL, keys.own), mine = 0;
+    if (m != 0 || takes_part<V>(z)) {  // a key, or NaN alone
       ++live;
-      Keys<V> keys;
-      keys.begin(z);
-      uint32_t m = __reduce_max_sync(FULL, keys.own), mine = 0;
       const float zmax = m ? of_key(m) : -INFINITY;
       const float inv = softmax<V>(z, zmax, e);
 #pragma unroll
@@ -611,16 +618,16 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
       sel = 0.0f;
     }
     if (t + warps_all < a.T) load(t + warps_all);
-    if (!takes_part<V>(z)) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, key_of(z[i]));
+    m = __reduce_max_sync(FULL, m);
+    if (m == 0 && !takes_part<V>(z)) {
 #pragma unroll
       for (int i = 0; i < V; ++i) e[i] = 0.0f;
       store_token<V>(a, b.dlogits, t, e);
       continue;
     }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) m = max(m, key_of(z[i]));
-    m = __reduce_max_sync(FULL, m);
     const float zmax = m ? of_key(m) : -INFINITY;
     const float inv = softmax<V>(z, zmax, e);
     // the chosen experts' share, in the lane that holds the choice
