@@ -12,7 +12,9 @@
 //
 // Both passes are bound by HBM: a row is read once, held in registers as
 // 16-byte vectors (8 features a thread and vector) and written once.  The row
-// sums are held in 32 bits and reduced in a fixed order.
+// sums are held in 32 bits and reduced in a fixed order.  Of 64 Mi elements the
+// 8-bit output with residual takes 0.88 to 1.02 of the copy rate from 128 to
+// 16384 features, the backward 0.82 to 1.09, the bf16 output alone 0.81 to 1.0.
 #include "common.cuh"
 
 namespace gl {
@@ -32,7 +34,6 @@ struct FwdArgs {
   float* rstd;        // or null
   int64_t M;
   int nvec;           // K / 8
-  int w32;
   float inv_k, eps;
 };
 
@@ -42,30 +43,53 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight features as four pairs: the arithmetic runs on packed f32x2
+// instructions, without which a row of 7168 with its 8-bit output costs twice
+// the issue slots and runs below HBM's rate at the clocks of a power-capped
+// part (143 us against 126 for 16384 rows).
+struct F8 {
+  float2 p[4];
+};
+
+__device__ __forceinline__ F8 unpack8(const uint4& u) {
+  return {{bf16x2_to_f32x2(u.x), bf16x2_to_f32x2(u.y), bf16x2_to_f32x2(u.z), bf16x2_to_f32x2(u.w)}};
+}
+
+__device__ __forceinline__ uint4 pack8(const F8& f) {
+  return make_uint4(pack_bf16x2(f.p[0].x, f.p[0].y), pack_bf16x2(f.p[1].x, f.p[1].y),
+                    pack_bf16x2(f.p[2].x, f.p[2].y), pack_bf16x2(f.p[3].x, f.p[3].y));
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ F8 mul8(const F8& a, const F8& b) {
+  F8 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = bf16x2_to_f32x2(w[i]);
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
+  for (int j = 0; j < 4; ++j) r.p[j] = __fmul2_rn(a.p[j], b.p[j]);
+  return r;
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                    pack_bf16x2(f[6], f[7]));
+__device__ __forceinline__ F8 scale8(const F8& a, float v) {
+  F8 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.p[j] = __fmul2_rn(a.p[j], both(v));
+  return r;
 }
 
-__device__ __forceinline__ void load_w8(const void* w, int w32, int vec, float (&f)[8]) {
-  if (w32) {
+// acc += a * b, pair by pair
+__device__ __forceinline__ void dot8(const F8& a, const F8& b, float2& acc) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = __ffma2_rn(a.p[j], b.p[j], acc);
+}
+
+template <bool kW32>
+__device__ __forceinline__ F8 load_w8(const void* w, int vec) {
+  if (kW32) {
     const float4 a = __ldg(static_cast<const float4*>(w) + 2 * vec);
     const float4 b = __ldg(static_cast<const float4*>(w) + 2 * vec + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    unpack8(__ldg(static_cast<const uint4*>(w) + vec), f);
+    return {{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
   }
+  return unpack8(__ldg(static_cast<const uint4*>(w) + vec));
 }
 
 // Sum over the threads of a row: L lanes of a warp, or (L = 0) the CTA's warps
@@ -86,9 +110,11 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 }
 
 // V vectors a thread.  L lanes a row (16 up to 128 features, a warp up to 1024),
-// SMALL_T threads a CTA; L = 0: a CTA per row.
-template <int V, int L>
-__global__ void __launch_bounds__(L ? SMALL_T : 1024) rms_norm_fwd_kernel(const FwdArgs a) {
+// SMALL_T threads a CTA; L = 0: a CTA per row, in 32 registers with two vectors
+// (h is kept packed and unpacked again), so that 2048 threads fit an SM: 7168
+// features 73 us for 9362 rows, 78 with 38 registers.
+template <int V, int L, bool kQuant, bool kW32>
+__global__ void __launch_bounds__(L ? SMALL_T : 1024, L == 0 && V == 2 ? 2 : 1) rms_norm_fwd_kernel(const FwdArgs a) {
   constexpr int LL = L ? L : 1;
   __shared__ float part[32];
   const int64_t row = L ? static_cast<int64_t>(blockIdx.x) * (SMALL_T / LL) + threadIdx.x / LL
@@ -109,65 +135,59 @@ __global__ void __launch_bounds__(L ? SMALL_T : 1024) rms_norm_fwd_kernel(const 
     xv[i] = vec < nvec ? a.x[base + vec] : make_uint4(0, 0, 0, 0);
     if (a.res) rv[i] = vec < nvec ? a.res[base + vec] : make_uint4(0, 0, 0, 0);
   }
-  float sum = 0.0f;
+  float2 sum2 = both(0.0f);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int vec = tid + i * step;
-    float f[8];
-    unpack8(xv[i], f);
+    F8 h = unpack8(xv[i]);
     if (a.res) {
-      float g[8];
-      unpack8(rv[i], g);
+      const F8 g = unpack8(rv[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] += g[j];
-      xv[i] = pack8(f);  // the sum as it is stored: the one rounding of h
+      for (int j = 0; j < 4; ++j) h.p[j] = __fadd2_rn(h.p[j], g.p[j]);
+      xv[i] = pack8(h);  // the sum as it is stored: the one rounding of h
       if (vec < nvec) a.h[base + vec] = xv[i];
-      unpack8(xv[i], f);
+      h = unpack8(xv[i]);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
+    dot8(h, h, sum2);
   }
-  sum = row_sum<L>(sum, part);
+  const float sum = row_sum<L>(sum2.x + sum2.y, part);
   const float r = rsqrtf(fmaf(sum, a.inv_k, a.eps));
   if (a.rstd && tid == 0 && live) a.rstd[row] = r;
 
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int vec = tid + i * step;
-    float f[8], w[8];
-    if (vec < nvec) {
-      unpack8(xv[i], f);
-      load_w8(a.w, a.w32, vec, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
+    const bool in = vec < nvec;
+    F8 f = scale8(unpack8(xv[i]), r);
+    if (in) {  // past the row all are 0
+      f = mul8(f, load_w8<kW32>(a.w, vec));
       if (a.y) a.y[base + vec] = pack8(f);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = 0.0f;
     }
-    if (a.q) {
+    if (kQuant) {
       // a block of 128 features is a half-warp's vectors (nvec % 16 == 0, so
       // a half-warp is inside the row or past it as a whole)
       float m = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]));
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(f.p[j].x), fabsf(f.p[j].y)));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      const float s = m == 0.0f ? 1.0f : m / 448.0f;
-      if (vec < nvec) {
-        // one division per block; blocks whose reciprocal would overflow (or
-        // whose maximum is infinite) divide each element
-        if (s >= 0x1p-100f && s <= 3.40282347e38f) {
-          const float inv = 1.0f / s;
+      float s;
+      if (m == 0.0f || (m >= 0x1p-90f && m <= 3.40282347e38f)) {
+        // m / 448 correctly rounded (Markstein: the rounded product with the
+        // rounded reciprocal, then one correction), its reciprocal to 1 ulp
+        constexpr float R = 1.0f / 448.0f;
+        s = m * R;
+        s = m == 0.0f ? 1.0f : fmaf(fmaf(-s, 448.0f, m), R, s);
+        f = scale8(f, __fdividef(1.0f, s));
+      } else {  // tiny or infinite: each element divided
+        s = m / 448.0f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= inv;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] /= s;
-        }
+        for (int j = 0; j < 4; ++j) f.p[j] = make_float2(f.p[j].x / s, f.p[j].y / s);
+      }
+      if (in) {
         uint32_t p[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = cvt_e4m3x2(f[2 * j], f[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) p[j] = cvt_e4m3x2(f.p[j].x, f.p[j].y);
         a.q[base + vec] = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
         if ((tid & 15) == 0) a.s[row * (a.nvec >> 4) + (vec >> 4)] = s;
       }
@@ -185,20 +205,21 @@ struct BwdArgs {
   float* part;        // fp32 [gridDim.x, K]: each CTA's share of dw
   int64_t M;
   int nvec;
-  int w32;
   float inv_k;
 };
 
 // A persistent CTA takes rows blockIdx.x, + gridDim.x, ... (L lanes each, or L =
-// 0: the CTA one row at a time) and keeps its columns' share of dw in registers.  dy and h of the next
-// row are loaded while this row's sum is under way (where MAX_T leaves the
-// registers), dh, which only dx needs, with the row itself.
-template <int V, int L, int MAX_T, int CTAS>
+// 0: the CTA one row at a time) and keeps its columns' share of dw in registers.
+// dy and h of the next row are loaded while this row's sum is under way, dh,
+// which only dx needs, with the row itself (4099 x 4096: 28 us without).  Above
+// 6144 features a second CTA on the SM is worth more than those registers (7168:
+// 88 us for 9362 rows, 98 with one CTA and loads ahead).
+template <int V, int L, int MAX_T, int CTAS, bool kW32>
 __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs a) {
-  constexpr bool kAhead = MAX_T <= 512;
+  constexpr bool kAhead = MAX_T <= 384;
   constexpr int LL = L ? L : 1, ROWS = L ? SMALL_T / LL : 1;
   __shared__ float part[2][32];
-  __shared__ float cross[ROWS][L ? L * V * 8 : 1];
+  __shared__ __align__(16) float cross[ROWS][L ? L * V * 8 : 2];
   const int tid = L ? threadIdx.x % LL : threadIdx.x;
   const int step = L ? L : blockDim.x;
   const int64_t rows_step = static_cast<int64_t>(gridDim.x) * ROWS;
@@ -213,7 +234,11 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
       hn[i] = in ? __ldg(a.h + r * a.nvec + vec) : make_uint4(0, 0, 0, 0);
     }
   };
-  float dw[V][8] = {};
+  F8 dw[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dw[i].p[j] = both(0.0f);
   if (kAhead) load(row);
   // as many rounds for every lane of a warp (rows may end inside one)
   const int64_t rounds = (a.M - static_cast<int64_t>(blockIdx.x) * ROWS + rows_step - 1) / rows_step;
@@ -232,37 +257,29 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
       dv[i] = a.dh && vec < nvec ? __ldg(a.dh + base + vec) : make_uint4(0, 0, 0, 0);
     }
     if (kAhead) load(row + rows_step);
-    float c = 0.0f;
+    float2 c2 = both(0.0f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int vec = tid + i * step;
       if (vec < nvec) {
-        float g[8], h[8], w[8];
-        unpack8(gv[i], g);
-        unpack8(hv[i], h);
-        load_w8(a.w, a.w32, vec, w);
+        const F8 g = unpack8(gv[i]), xh = scale8(unpack8(hv[i]), r);
+        dot8(mul8(g, load_w8<kW32>(a.w, vec)), xh, c2);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float xh = h[j] * r;
-          c = fmaf(g[j] * w[j], xh, c);
-          dw[i][j] = fmaf(g[j], xh, dw[i][j]);
-        }
+        for (int j = 0; j < 4; ++j) dw[i].p[j] = __ffma2_rn(g.p[j], xh.p[j], dw[i].p[j]);
       }
     }
     // two sets of slots: a warp may reach the next row's sum while another
     // still reads this one's
-    c = row_sum<L>(c, part[it]) * a.inv_k;
+    const float c = row_sum<L>(c2.x + c2.y, part[it]) * a.inv_k;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int vec = tid + i * step;
       if (vec < nvec) {
-        float g[8], h[8], d[8], w[8];
-        unpack8(gv[i], g);
-        unpack8(hv[i], h);
-        unpack8(dv[i], d);
-        load_w8(a.w, a.w32, vec, w);
+        const F8 u = mul8(unpack8(gv[i]), load_w8<kW32>(a.w, vec)), xh = scale8(unpack8(hv[i]), r);
+        F8 d = unpack8(dv[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = fmaf(r, fmaf(-h[j] * r, c, g[j] * w[j]), d[j]);
+        for (int j = 0; j < 4; ++j)
+          d.p[j] = __ffma2_rn(both(r), __ffma2_rn(xh.p[j], both(-c), u.p[j]), d.p[j]);
         a.dx[base + vec] = pack8(d);
       }
     }
@@ -272,7 +289,8 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cross[threadIdx.x / LL][(tid + i * L) * 8 + j] = dw[i][j];
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float2*>(&cross[threadIdx.x / LL][(tid + i * L) * 8 + 2 * j]) = dw[i].p[j];
     __syncthreads();
     for (int k = threadIdx.x; k < a.nvec * 8; k += blockDim.x) {
       float s = 0.0f;
@@ -285,8 +303,10 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
     for (int i = 0; i < V; ++i) {
       const int vec = tid + i * step;
       if (vec < a.nvec) {
-        reinterpret_cast<float4*>(out)[2 * vec] = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
-        reinterpret_cast<float4*>(out)[2 * vec + 1] = make_float4(dw[i][4], dw[i][5], dw[i][6], dw[i][7]);
+        reinterpret_cast<float4*>(out)[2 * vec] =
+            make_float4(dw[i].p[0].x, dw[i].p[0].y, dw[i].p[1].x, dw[i].p[1].y);
+        reinterpret_cast<float4*>(out)[2 * vec + 1] =
+            make_float4(dw[i].p[2].x, dw[i].p[2].y, dw[i].p[3].x, dw[i].p[3].y);
       }
     }
   }
@@ -328,7 +348,7 @@ BwdShape bwd_shape(int nvec) {
   if (nvec <= 32) return {SMALL_T, SMALL_T / 32, 4};
   if (nvec <= 64) return {SMALL_T, SMALL_T / 32, 3};
   const int t = row_threads(nvec, 2);
-  return {t, 1, t <= 256 ? 768 / t : t <= 384 ? 2 : 1};
+  return {t, 1, t <= 256 ? 768 / t : t <= 512 ? 2 : 1};
 }
 
 // CTAs of the backward (also the rows of its workspace).
@@ -336,6 +356,47 @@ int bwd_ctas(int64_t M, int nvec, int num_sms) {
   const BwdShape b = bwd_shape(nvec);
   const int64_t need = (M + b.rows - 1) / b.rows, most = static_cast<int64_t>(b.per_sm) * num_sms;
   return static_cast<int>(need < most ? need : most);
+}
+
+template <bool kQuant, bool kW32>
+void launch_fwd(const FwdArgs& a, cudaStream_t st) {
+  const int n = a.nvec;
+  const auto ctas = [&](int lanes) {
+    return static_cast<unsigned>((a.M + SMALL_T / lanes - 1) / (SMALL_T / lanes));
+  };
+  const unsigned rows = static_cast<unsigned>(a.M);
+  if (n <= 16)
+    rms_norm_fwd_kernel<1, 16, kQuant, kW32><<<ctas(16), SMALL_T, 0, st>>>(a);
+  else if (n <= 32)
+    rms_norm_fwd_kernel<1, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 64)
+    rms_norm_fwd_kernel<2, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 128)
+    rms_norm_fwd_kernel<4, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+  else if (n <= 1024)
+    rms_norm_fwd_kernel<2, 0, kQuant, kW32><<<rows, row_threads(n, 2), 0, st>>>(a);
+  else  // CTAs of half the threads, more of them an SM: K = 12288 in bf16 59 -> 47 us (5461 rows)
+    rms_norm_fwd_kernel<4, 0, kQuant, kW32><<<rows, row_threads(n, 4), 0, st>>>(a);
+}
+
+// t: threads of a row that a CTA takes.  The shapes are bwd_shape's.
+template <bool kW32>
+void launch_bwd(const BwdArgs& a, int ctas, int t, cudaStream_t st) {
+  const int n = a.nvec;
+  if (n <= 16)
+    rms_norm_bwd_kernel<1, 16, SMALL_T, 4, kW32><<<ctas, SMALL_T, 0, st>>>(a);
+  else if (n <= 32)
+    rms_norm_bwd_kernel<1, 32, SMALL_T, 4, kW32><<<ctas, SMALL_T, 0, st>>>(a);
+  else if (n <= 64)
+    rms_norm_bwd_kernel<2, 32, SMALL_T, 3, kW32><<<ctas, SMALL_T, 0, st>>>(a);
+  else if (t <= 256)
+    rms_norm_bwd_kernel<2, 0, 256, 3, kW32><<<ctas, t, 0, st>>>(a);
+  else if (t <= 384)
+    rms_norm_bwd_kernel<2, 0, 384, 2, kW32><<<ctas, t, 0, st>>>(a);
+  else if (t <= 512)
+    rms_norm_bwd_kernel<2, 0, 512, 2, kW32><<<ctas, t, 0, st>>>(a);
+  else
+    rms_norm_bwd_kernel<2, 0, 1024, 1, kW32><<<ctas, t, 0, st>>>(a);
 }
 
 }  // namespace rms
@@ -355,21 +416,11 @@ int gl_launch_rms_norm_fwd(const void* x, const void* residual, const void* weig
   using namespace gl::rms;
   FwdArgs a{static_cast<const uint4*>(x), static_cast<const uint4*>(residual), weight,
             static_cast<uint4*>(h), static_cast<uint4*>(y), static_cast<uint2*>(q), s, rstd, M,
-            static_cast<int>(K / 8), w32, 1.0f / static_cast<float>(K), eps};
-  const int n = a.nvec;
-  const auto ctas = [&](int lanes) { return static_cast<unsigned>((M + SMALL_T / lanes - 1) / (SMALL_T / lanes)); };
-  if (n <= 16)
-    rms_norm_fwd_kernel<1, 16><<<ctas(16), SMALL_T, 0, st>>>(a);
-  else if (n <= 32)
-    rms_norm_fwd_kernel<1, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
-  else if (n <= 64)
-    rms_norm_fwd_kernel<2, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
-  else if (n <= 128)
-    rms_norm_fwd_kernel<4, 32><<<ctas(32), SMALL_T, 0, st>>>(a);
-  else if (n <= 1024)
-    rms_norm_fwd_kernel<2, 0><<<static_cast<unsigned>(M), row_threads(n, 2), 0, st>>>(a);
-  else  // two CTAs of half the threads an SM more: K = 12288 in bf16 59 -> 47 us (5461 rows)
-    rms_norm_fwd_kernel<4, 0><<<static_cast<unsigned>(M), row_threads(n, 4), 0, st>>>(a);
+            static_cast<int>(K / 8), 1.0f / static_cast<float>(K), eps};
+  if (q)
+    w32 ? launch_fwd<true, true>(a, st) : launch_fwd<true, false>(a, st);
+  else
+    w32 ? launch_fwd<false, true>(a, st) : launch_fwd<false, false>(a, st);
   return launched(why);
 }
 
@@ -384,23 +435,10 @@ int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const 
   const int n = static_cast<int>(K / 8), t = row_threads(n, 2);
   const int ctas = bwd_ctas(M, n, num_sms);
   const BwdArgs a{static_cast<const uint4*>(dy), static_cast<const uint4*>(dh), static_cast<const uint4*>(h),
-                  weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, n, w32,
+                  weight, rstd, static_cast<uint4*>(dx), static_cast<float*>(ws), M, n,
                   1.0f / static_cast<float>(K)};
   if (ctas > 0) {  // no rows: dw is a sum over nothing
-    if (n <= 16)
-      rms_norm_bwd_kernel<1, 16, SMALL_T, 4><<<ctas, SMALL_T, 0, st>>>(a);
-    else if (n <= 32)
-      rms_norm_bwd_kernel<1, 32, SMALL_T, 4><<<ctas, SMALL_T, 0, st>>>(a);
-    else if (n <= 64)
-      rms_norm_bwd_kernel<2, 32, SMALL_T, 3><<<ctas, SMALL_T, 0, st>>>(a);
-    else if (t <= 256)
-      rms_norm_bwd_kernel<2, 0, 256, 3><<<ctas, t, 0, st>>>(a);
-    else if (t <= 384)
-      rms_norm_bwd_kernel<2, 0, 384, 2><<<ctas, t, 0, st>>>(a);
-    else if (t <= 512)
-      rms_norm_bwd_kernel<2, 0, 512, 1><<<ctas, t, 0, st>>>(a);
-    else
-      rms_norm_bwd_kernel<2, 0, 1024, 1><<<ctas, t, 0, st>>>(a);
+    w32 ? launch_bwd<true>(a, ctas, t, st) : launch_bwd<false>(a, ctas, t, st);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
       *why = cudaGetErrorString(e);
