@@ -34,6 +34,10 @@
 //     exact (values 2^38 below the largest lose bits far under the sum's
 //     rounding), and scaled back where the block's fp32 sum meets the weights'
 //     scale.
+// Measured (K 7168, N 2048, 128 groups): 128 rows in 44 groups 65 us, 5.3 TB/s of
+// weights and scales (60 us without finishing split jobs, 55 us without the
+// sums); 8 rows in 8 groups 18 us (12 us of loads; the first unit lands 2 us
+// after the launch, split jobs are finished 2 us after the last).
 #include "common.cuh"
 
 #include <cuda_fp16.h>
