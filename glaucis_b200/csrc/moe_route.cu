@@ -327,8 +327,9 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, RouteShared<
       }
       if (id >= 0) p = exp_of(of_key(mine) - zmax) * inv;
       if (a.renorm) {
+        // correctly rounded: a single choice has weight 1 and no gradient
         const float s = warp_sum(p);
-        if (id >= 0) p = __fdividef(p, s);
+        if (id >= 0) p /= s;
       }
     }
     if (lane < a.k) {

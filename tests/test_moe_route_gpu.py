@@ -202,6 +202,15 @@ def test_backward(cuda, T, E, k, bf16, renorm):
     assert (np.abs(a + b - dz) <= 2 * tol + half).all()
 
 
+@pytest.mark.parametrize("T,E", [(50, 7), (3000, 128)])
+def test_a_single_choice_has_weight_one_and_no_gradient(cuda, T, E):
+    logits = _logits(cuda, T, E, False, seed=23)
+    r = ops.moe_route_fwd(logits, 1)
+    assert (r.weights == 1).all()
+    dw = torch.randn((T, 1), device=cuda, generator=torch.Generator(device=cuda).manual_seed(1)) * 1e3
+    assert (ops.moe_route_bwd(logits, r, dw, None) == 0).all()
+
+
 def test_gradient_against_differences(cuda):
     T, E, k = 24, 20, 3
     logits = _logits(cuda, T, E, False, seed=17)
