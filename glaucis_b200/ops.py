@@ -24,14 +24,16 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-# The current stream's handle without building a Stream object (3 us a call).
+# The current stream's handle without building a Stream object (3 us a call);
+# CUDA is initialised where there is a tensor to launch on.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream() -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream().cuda_stream
-    return _raw_stream(torch.cuda.current_device())
+    return _raw_stream(_current_device())
 
 
 def _need_cuda(*ts: Optional[torch.Tensor]) -> None:
@@ -644,16 +646,21 @@ def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]):
         if t is not None and (t.get_device() != dev or not t.is_contiguous()):
             _need_cuda(t)
             raise ValueError(f"all tensors of a call must be on one device, got {first.device} and {t.device}")
-    return _NO_GUARD if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NO_GUARD if dev == _current_device() else torch.cuda.device(dev)
 
 
 def _new(like: torch.Tensor, t: Optional[torch.Tensor], shape, dtype: torch.dtype, name: str) -> torch.Tensor:
-    """_out on `like`'s device (empty_like, the cheapest call, where it will do)."""
+    """_out on `like`'s device."""
     if t is not None:
         return _out(t, shape, dtype, like.device, name)
-    if like.shape == shape:
-        return torch.empty_like(like) if like.dtype == dtype else torch.empty_like(like, dtype=dtype)
     return torch.empty(*shape, dtype=dtype, device=like.device)
+
+
+def _new_like(like: torch.Tensor, t: Optional[torch.Tensor], dtype: torch.dtype, name: str) -> torch.Tensor:
+    """_out of `like`'s shape on its device."""
+    if t is not None:
+        return _out(t, like.shape, dtype, like.device, name)
+    return torch.empty_like(like, dtype=dtype)
 
 
 class RMSNormForward(NamedTuple):
@@ -668,12 +675,13 @@ class RMSNormForward(NamedTuple):
 
 
 def _rms_check(x, weight, residual):
-    if x.dtype != torch.bfloat16 or x.dim() != 2:
+    shape = x.shape
+    if x.dtype != torch.bfloat16 or len(shape) != 2:
         raise ValueError("x must be a 2-D bf16 tensor")
-    M, K = x.shape
-    if weight.dtype not in (torch.bfloat16, torch.float32) or tuple(weight.shape) != (K,):
+    M, K = shape
+    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.shape != shape[1:]:
         raise ValueError("weight must be bf16 or fp32 [K]")
-    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape):
+    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != shape):
         raise ValueError("residual must be bf16 of x's shape")
     return M, K
 
@@ -704,10 +712,10 @@ def rms_norm_quant_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
         M, K = _rms_check(x, weight, residual)
         if h is not None and residual is None:
             raise ValueError("h goes with a residual")
-        q = _new(x, q, (M, K), FP8, "q")
+        q = _new_like(x, q, FP8, "q")
         s = _new(x, s, (M, K // TILE), torch.float32, "s")
         if residual is not None:
-            h = _new(x, h, (M, K), torch.bfloat16, "h")
+            h = _new_like(x, h, torch.bfloat16, "h")
         _rms_norm(x, weight, eps, residual, h, None, q, s, None)
     return (q, s) if residual is None else (q, s, h)
 
@@ -724,12 +732,12 @@ def rms_norm_fwd(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
         M, K = _rms_check(x, weight, residual)
         if h is not None and residual is None:
             raise ValueError("h goes with a residual")
-        y = _new(x, y, (M, K), torch.bfloat16, "y")
-        h = _new(x, h, (M, K), torch.bfloat16, "h") if residual is not None else x
+        y = _new_like(x, y, torch.bfloat16, "y")
+        h = _new_like(x, h, torch.bfloat16, "h") if residual is not None else x
         q = s = None
         if output_quant:
-            q = x.new_empty((M, K), dtype=FP8)
-            s = x.new_empty((M, K // TILE), dtype=torch.float32)
+            q = torch.empty_like(x, dtype=FP8)
+            s = torch.empty(M, K // TILE, dtype=torch.float32, device=x.device)
         rstd = x.new_empty(M, dtype=torch.float32)
         _rms_norm(x, weight, eps, residual, h, y, q, s, rstd)
     return RMSNormForward(y, h, q, s, rstd)
