@@ -474,29 +474,22 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
   }
 
   if (warp > WARPS) {
-    // ---- rows of x: a warp takes the units of one stage, the next one's rows
-    // loaded before this one's are stored ----
+    // ---- rows of x: a warp takes the units of one stage; a unit's rows are on
+    // their way while the stage is still in use ----
     const int st = warp - WARPS - 1;
     if (st >= units) return;
     walk.begin(a, u0);
     for (int i = 0; i < st; ++i) walk.advance(a, true);
-    XRows cur;
-    cur.load(a, walk.tile, walk.block);
     uint32_t phase = 1;  // the first round is free
     for (int n = st; n < units; n += S) {
-      const int nrows = walk.tile.nrows;
-      XRows next;
-      if (n + S < units) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) walk.advance(a, true);
-        next.load(a, walk.tile, walk.block);
-      }
+      XRows rows;
+      rows.load(a, walk.tile, walk.block);
       if (n >= S && !mbar_wait(&ct.empty[st], phase, ab)) return;
-      cur.store(smem + st * STAGE_BYTES + X_OFF, nrows);
+      rows.store(smem + st * STAGE_BYTES + X_OFF, walk.tile.nrows);
       __syncwarp();
       if (lane == 0) mbar_arrive(&ct.full[st]);
-      cur = next;
       phase ^= 1;
+      for (int i = 1; i <= S; ++i) walk.advance(a, n + S < units);
     }
     return;
   }
