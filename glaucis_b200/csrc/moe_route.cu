@@ -24,6 +24,8 @@
 // gradient 40 us; 32768 tokens of 256 experts 36 us, 8192 of 1024 80 us.
 #include "common.cuh"
 
+#include <atomic>
+
 namespace gl {
 namespace route {
 
@@ -708,11 +710,15 @@ int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
 template <int V>
 int bwd(const Args& a, const BwdArgs& b, int num_sms, cudaStream_t st, const char** why) {
   const int64_t need = (a.T + 7) / 8;
-  int per_sm = 0;
-  cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, route_bwd_kernel<V>, 256, 0);
-  if (q != cudaSuccess) {
-    *why = cudaGetErrorString(q);
-    return -2;
+  static std::atomic<int> fit{0};  // CTAs of an SM, the same on every B200
+  int per_sm = fit.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    const cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, route_bwd_kernel<V>, 256, 0);
+    if (q != cudaSuccess) {
+      *why = cudaGetErrorString(q);
+      return -2;
+    }
+    fit.store(per_sm, std::memory_order_relaxed);
   }
   const int64_t most = static_cast<int64_t>(num_sms) * per_sm;
   route_bwd_kernel<V><<<static_cast<unsigned>(need < most ? need : most), 256, 0, st>>>(a, b);

@@ -263,6 +263,25 @@ def test_the_same_every_time_and_on_two_streams(cuda, T):
             assert all(torch.equal(a, b) for a, b in zip(r[:6], want[i][:6]))
 
 
+def test_offsets_past_32_bits(cuda):
+    T, E, k = 2_200_000, 1024, 4  # 2.25e9 logits
+    logits = torch.zeros((T, E), dtype=torch.bfloat16, device=cuda)
+    logits[:, 3:7] = 1
+    logits[-500:] = _logits(cuda, 500, E, True, seed=29)
+    r = ops.moe_route_fwd(logits, k)
+    tail = ops.moe_route_fwd(logits[-500:].clone(), k)
+    assert torch.equal(r.ids[-500:], tail.ids) and torch.equal(r.weights[-500:], tail.weights)
+    want = torch.bincount(r.ids.reshape(-1).long(), minlength=E).int()
+    assert torch.equal(r.counts, want) and (r.ids[:-500] == torch.arange(3, 7, device=cuda)).all()
+    rows = torch.zeros(T * k, dtype=torch.bool, device=cuda)
+    rows[r.pos.reshape(-1).long()] = True
+    assert rows.all()  # every row once
+    start = want.cumsum(0) - want
+    assert ((r.pos >= start[r.ids.long()]) & (r.pos < (start + want)[r.ids.long()])).all()
+    dl = ops.moe_route_bwd(logits, r, torch.ones_like(r.weights), None)
+    assert torch.isfinite(dl[-500:].float()).all()
+
+
 def test_refusals(cuda):
     z = torch.zeros((4, 16), device=cuda)
     for bad in (z.half(), z[0], z.double()):

@@ -210,6 +210,22 @@ def test_rows_of_a_larger_tensor_and_another_stream(cuda):
     assert torch.equal(out[7:20], want) and (out[:7] == 3).all() and (out[20:] == 3).all()
 
 
+def test_offsets_past_32_bits(cuda):
+    M, K = 600_000, 4096  # 2.46e9 elements
+    x = torch.ones((M, K), dtype=BF16, device=cuda)
+    tail, _, w, _, _ = _inputs(cuda, 200, K, False, True, seed=10)
+    x[-200:] = tail
+    q, s = ops.rms_norm_quant_1x128(x, w)
+    want_q, want_s = ops.rms_norm_quant_1x128(tail, w)
+    assert torch.equal(q[-200:].view(torch.uint8), want_q.view(torch.uint8)) and torch.equal(s[-200:], want_s)
+    del q, s
+    f = ops.rms_norm_fwd(x, w)
+    want = ops.rms_norm_fwd(tail, w)
+    assert torch.equal(f.y[-200:], want.y) and torch.equal(f.rstd[-200:], want.rstd)
+    dx, _ = ops.rms_norm_bwd(f.y, f.h, w, f.rstd)
+    assert torch.equal(dx[-200:], ops.rms_norm_bwd(want.y, tail, w, want.rstd)[0])
+
+
 def test_refusals(cuda):
     x, res, w, dy, _ = _inputs(cuda, 4, 256, True, False)
     with pytest.raises(ValueError, match="2-D bf16"):
