@@ -275,13 +275,14 @@ __global__ void __launch_bounds__(256, V <= 4 ? 4 : 2) combine_bwd_kernel(const 
         for (int i = 0; i < V; ++i) {
           const int vec = threadIdx.x + i * blockDim.x;
           if (vec < a.nvec) {
-            float f[8], g[8];
+            float f[8], g[8], sum = 0.0f;
             v[i].floats(f);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              dot = fmaf(d[i][e], f[e], dot);
+              sum = fmaf(d[i][e], f[e], sum);
               g[e] = w * d[i][e];
             }
+            dot += sum;
             if (kF32) {
               float4* o = static_cast<float4*>(a.dy) + 2 * (p * a.nvec + vec);
               o[0] = make_float4(g[0], g[1], g[2], g[3]);
@@ -373,9 +374,18 @@ int gl_launch_moe_combine_bwd(const void* dout, const void* y, int y_f32, const 
   const CombineBwdArgs a{static_cast<const uint4*>(dout), y, pos, weights, group_sizes, T, rows,
                          static_cast<int>(k), static_cast<int>(G), static_cast<int>(K / 8), dy, dweights,
                          err};
-  const int v = (a.nvec + 255) / 256;
-  const int threads = a.nvec < 256 ? (a.nvec + 31) / 32 * 32 : 256;
-  const int64_t most = 8 * static_cast<int64_t>(num_sms);
+  // A thread takes 4 vectors of 8 (2 of fp32) where there are tokens enough to
+  // fill the SMs: small CTAs and more loads in flight.  us against 256 threads
+  // with as many vectors as the row then needs: 16387 tokens, topk 2, K 4096: 103
+  // (120); 4096, 8, 2048: 54 (72); 8192, 4, 512: 18 (33).  With fewer tokens
+  // a wide CTA is the shorter path (33 tokens, topk 8, K 4096: 6.5 against 8.2);
+  // above 160 threads whole CTAs of 256 were faster (4096, 8, 7168: 168 against
+  // 186 with 224).
+  const int per = T <= 4 * static_cast<int64_t>(num_sms) ? 1 : y_f32 ? 2 : 4;
+  const int need = ((a.nvec + per - 1) / per + 31) / 32 * 32;
+  const int threads = need < 192 ? need : 256;
+  const int v = (a.nvec + threads - 1) / threads;
+  const int64_t most = 2048 / threads * static_cast<int64_t>(num_sms);
   const unsigned ctas = static_cast<unsigned>(T < 1 ? 1 : T < most ? T : most);
   if (v <= 1)
     combine_bwd<1>(a, y_f32, ctas, threads, st);

@@ -33,7 +33,8 @@ def _rand(cuda, *shape, seed=0, dtype=BF16):
 
 
 SHAPES = [(1, 8, 1, 8), (1, 128, 8, 7168), (4, 128, 8, 7168), (37, 60, 4, 264), (130, 8, 2, 1024), (65, 64, 6, 2056),
-          (700, 256, 8, 512), (9, 40, 32, 4096), (2100, 8, 2, 4096), (3, 16, 3, 16384)]
+          (700, 256, 8, 512), (9, 40, 32, 4096), (2100, 8, 2, 4096), (3, 16, 3, 16384),
+          (600, 12, 3, 264), (650, 8, 2, 5120), (601, 8, 1, 16)]
 
 
 @pytest.mark.parametrize("T,E,k,K", SHAPES)
