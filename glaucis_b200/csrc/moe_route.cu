@@ -9,10 +9,10 @@
 // A warp takes a token, lane l holding the V experts from l V on: the softmax's
 // sums and the k rounds of the selection are warp reductions on registers.
 // Each lane keeps the largest of its own keys at hand, so a round is one
-// redux.max, a ballot whose lowest lane holds the lowest expert of that key,
-// and the winner's next key taking its place.  With E floats a token to read it
-// is bound by issuing these instructions, mostly integer ones (460 a token of
-// 128 experts and 8 choices), not by HBM.
+// redux.max for the key, a redux.min for the lowest expert that has it, and the
+// winner's next key taking its place.  With E floats a token to read it is bound
+// by issuing these instructions, mostly integer ones (440 a token of 128 experts
+// and 8 choices), not by HBM.
 //
 // Rows need the counts of all earlier tokens: each CTA takes consecutive tokens
 // and leaves its counts per expert, a second launch (not needed when one CTA
@@ -199,28 +199,19 @@ __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float 
 
 // A lane's keys and where they are, so that the largest is at hand and the next
 // takes its place when it is chosen.  Fours of consecutive experts are kept
-// sorted (equal keys in the experts' order), and the largest is that of the
-// fours' heads; of 16 and more, for which registers run short, it is looked for
-// again.
+// sorted (equal keys in the experts' order, which stands in a word, a byte
+// each), and the largest is that of the fours' heads; of 32, where the order of
+// eight fours costs more than it saves (84 us against 81 for 8192 tokens of 1024
+// experts; of 384: 42 against 52 for 16384), it is looked for again.
 template <int V>
 struct Keys {
-  static constexpr bool kSorted = V <= 8;
+  static constexpr bool kSorted = V <= 16;
   static constexpr int F = V < 4 ? V : 4, N = V / F;  // keys of a four, fours
   uint32_t key[V];
-  int at[V];  // kSorted: index of each; else at[0]: index of the largest
+  uint32_t at[kSorted ? N : 1];  // kSorted: a four's experts, a byte each; else index of the largest
   uint32_t own;
   int four;   // whose head it is
 
-  __device__ __forceinline__ void order(int i, int j) {  // i < j
-    if (key[j] > key[i]) {
-      const uint32_t k = key[i];
-      key[i] = key[j];
-      key[j] = k;
-      const int t = at[i];
-      at[i] = at[j];
-      at[j] = t;
-    }
-  }
   __device__ __forceinline__ void look() {
     own = key[0];
     if constexpr (kSorted) {
@@ -245,25 +236,38 @@ struct Keys {
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = key_of(z[i]);
     if constexpr (kSorted) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) at[i] = i;
       // exchange of neighbours only, which keeps equal keys in order
 #pragma unroll
-      for (int b = 0; b < V; b += F)
+      for (int b = 0; b < N; ++b) {
+        uint32_t x[F];
+#pragma unroll
+        for (int i = 0; i < F; ++i) x[i] = b * F + i;
 #pragma unroll
         for (int n = F - 1; n > 0; --n)
 #pragma unroll
-          for (int i = 0; i < n; ++i) order(b + i, b + i + 1);
+          for (int i = 0; i < n; ++i) {
+            uint32_t &p = key[b * F + i], &q = key[b * F + i + 1];
+            const bool swap = q > p;
+            const uint32_t k = swap ? p : q, t = swap ? x[i] : x[i + 1];
+            p = swap ? q : p;
+            x[i] = swap ? x[i + 1] : x[i];
+            q = k;
+            x[i + 1] = t;
+          }
+        at[b] = x[0];
+#pragma unroll
+        for (int i = 1; i < F; ++i) at[b] |= x[i] << (8 * i);
+      }
     }
     look();
   }
   __device__ __forceinline__ int expert() const {
-    int i = at[0];
+    uint32_t i = at[0];
     if constexpr (kSorted) {
 #pragma unroll
-      for (int n = 1; n < N; ++n) i = four == n ? at[n * F] : i;
+      for (int n = 1; n < N; ++n) i = four == n ? at[n] : i;
     }
-    return (threadIdx.x & 31) * V + i;
+    return i;
   }
   // Takes the largest away (in the lane with `won`).
   __device__ __forceinline__ void next(bool won) {
@@ -272,11 +276,9 @@ struct Keys {
       for (int n = 0; n < N; ++n) {
         if (won && (N == 1 || four == n)) {
 #pragma unroll
-          for (int i = n * F; i + 1 < (n + 1) * F; ++i) {
-            key[i] = key[i + 1];
-            at[i] = at[i + 1];
-          }
+          for (int i = n * F; i + 1 < (n + 1) * F; ++i) key[i] = key[i + 1];
           key[(n + 1) * F - 1] = 0;
+          at[n] >>= 8;
         }
       }
       look();
@@ -317,21 +319,23 @@ __device__ void route_tokens(const Args& a, int64_t t0, int64_t t1, RouteShared<
 #pragma unroll
       for (int i = 0; i < V; ++i) psum[i] = fmaf(e[i], inv, psum[i]);
       for (int j = 0; m != 0; ) {  // 0: nothing left to choose
-        const int src = __ffs(__ballot_sync(FULL, keys.own == m)) - 1;
-        const int at = __shfl_sync(FULL, keys.expert(), src);
+        const uint32_t x = keys.own == m ? lane * V + (keys.expert() & 255) : 0xffffu;
+        const uint32_t at = __reduce_min_sync(FULL, x);
         if (lane == j) {
           id = at;
           mine = m;
         }
         if (++j == a.k) break;
-        keys.next(lane == src);
+        keys.next(x == at);
         m = __reduce_max_sync(FULL, keys.own);
       }
       if (id >= 0) p = exp_of(of_key(mine) - zmax) * inv;
       if (a.renorm) {
-        // correctly rounded: a single choice has weight 1 and no gradient
+        // the quotient with its remainder put right (s is 2^-10 to 1): a single
+        // choice has weight 1 exactly and no gradient
         const float s = warp_sum(p);
-        if (id >= 0) p /= s;
+        const float r = __fdividef(1.0f, s), q = p * r;
+        if (id >= 0) p = fmaf(fmaf(-q, s, p), r, q);
       }
     }
     if (lane < a.k) {
@@ -484,8 +488,10 @@ __global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a
 }
 
 // First of two launches: the choices, and what the CTA adds to counts and loss.
+// Up to 128 experts it keeps to half of an SM's registers, so that the second
+// launch's CTAs start beside it (65536 tokens of 128: 45 us against 51).
 template <int V>
-__global__ void __launch_bounds__(32 * warps<V>()) route_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * warps<V>(), V <= 4 ? 2 : 1) route_kernel(const Args a) {
   __shared__ RouteShared<V> sh;
   cudaTriggerProgrammaticLaunchCompletion();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
