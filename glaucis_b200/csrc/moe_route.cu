@@ -673,10 +673,13 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
 // Warps of a forward CTA for E experts.
 int fwd_warps(int64_t E) { return E <= 256 ? warps<8>() : E <= 512 ? warps<16>() : warps<32>(); }
 
-// CTAs of the forward: one when its warps take every token in a few rounds
-// (a second launch costs more than those rounds), else one per SM at most.
-int fwd_ctas(int64_t T, int w, int num_sms) {
-  if (T <= 2 * w) return 1;
+// CTAs of the forward: one when a token each is enough for its warps, or two
+// with one or two choices each, else one per SM at most.  The second launch
+// costs less than a second round of 8 choices (64 tokens of 128 experts: 7.3 us
+// against 8.7), more than one of 2 (33 to 64 tokens of 8: 5.9 to 6.2 against 5.0
+// to 5.5).
+int fwd_ctas(int64_t T, int64_t k, int w, int num_sms) {
+  if (T <= (k <= 2 ? 2 * w : w)) return 1;
   const int64_t need = (T + w - 1) / w;
   const int most = num_sms < MAX_CTAS ? num_sms : MAX_CTAS;
   return static_cast<int>(need < most ? need : most);
@@ -685,7 +688,7 @@ int fwd_ctas(int64_t T, int w, int num_sms) {
 template <int V>
 int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
   Args a = a0;
-  const int ctas = fwd_ctas(a.T, warps<V>(), num_sms);
+  const int ctas = fwd_ctas(a.T, a.k, warps<V>(), num_sms);
   a.chunk = a.T > 0 ? (a.T + ctas - 1) / ctas : 1;
   cudaError_t e;
   if (ctas == 1) {
@@ -749,10 +752,11 @@ static int lane_experts(int64_t E) {
   return v;
 }
 
-// hist and psum of every CTA, then its number of routed tokens; none for one CTA.
+// hist and psum of every CTA, then its number of routed tokens; none for one
+// CTA whatever the number of choices.
 size_t gl_moe_route_ws_bytes(int64_t T, int64_t E) {
   using namespace gl::route;
-  if (fwd_ctas(T, fwd_warps(E), MAX_CTAS) == 1) return 0;
+  if (fwd_ctas(T, GL_MOE_MAX_TOPK, fwd_warps(E), MAX_CTAS) == 1) return 0;
   return static_cast<size_t>(MAX_CTAS) * (2 * static_cast<size_t>(E) + 1) * 4;
 }
 
