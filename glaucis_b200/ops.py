@@ -998,13 +998,13 @@ class _MoEDispatch(torch.autograd.Function):
 def moe_dispatch(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
                  rows: Optional[int] = None) -> torch.Tensor:
     """Rows of the tokens in expert order: out[pos[t, j]] = x[t] (bf16 [T, K])
-    for the pos and counts of moe_route (distinct rows below sum(group_sizes), a
-    negative one is skipped); the lhs of gmm_fp8_blockwise with group_sizes =
+    for the pos and counts of moe_route (rows 0 to sum(group_sizes) - 1, each of
+    one choice; a negative one is skipped); the lhs of gmm_fp8_blockwise with group_sizes =
     counts.  `rows` (default T * topk) is the number of output rows; those past
     sum(group_sizes) are zero.  Differentiable in x (bf16)."""
     if torch.is_grad_enabled() and x.requires_grad:
-        if x.dtype != torch.bfloat16:
-            raise ValueError("the differentiable moe_dispatch takes bf16")
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] > 16384:
+            raise ValueError("the differentiable moe_dispatch takes bf16 [T, K], K at most 16384")
         return _MoEDispatch.apply(x, pos, group_sizes, rows)
     return moe_dispatch_fwd(x, pos, group_sizes, rows)
 

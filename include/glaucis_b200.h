@@ -403,8 +403,9 @@ int gl_moe_route_bwd(const void* logits, int logits_f32, const void* mask, const
  * Rows into expert order: out[pos[t, j]] = x[t] for every pos >= 0.
  *   x            [T, row_bytes] (any type; row_bytes a multiple of 16)
  *   s            fp32 [T, scales] moved alongside into out_s, or both NULL
- *   pos          int32 [T, topk] as gl_moe_route_fwd writes it: distinct rows
- *                below sum(group_sizes); a negative one is skipped
+ *   pos          int32 [T, topk] as gl_moe_route_fwd writes it: the rows below
+ *                sum(group_sizes), each of one choice (one that no choice names
+ *                is left as it is); a negative one is skipped
  *   group_sizes  int32 [G], 1 <= G <= 1024
  *   out, out_s   [rows, ...]; rows at or past sum(group_sizes) are set to
  *                zero, their scales to 1 (the pair of a zero block)

@@ -232,3 +232,5 @@ def test_refusals(cuda):
         ops.moe_dispatch(x, torch.zeros((T, 33), dtype=torch.int32, device=cuda), sizes)
     with pytest.raises(ValueError, match="takes bf16"):
         ops.moe_dispatch(x.float().requires_grad_(), pos, sizes)
+    with pytest.raises(ValueError, match="at most 16384"):  # which its gradient could not take
+        ops.moe_dispatch(_rand(cuda, T, 16512).requires_grad_(), pos, sizes)
