@@ -21,8 +21,8 @@
 // warps and CTAs: results do not depend on timing.
 //
 // Measured, 128 experts, top 8: 3 tokens 4.4 us, 4096 9.7 us, 32771 with the
-// gradient 38 us; 32768 tokens of 256 experts 37 us, 16384 of 384 43 us, 8192 of
-// 1024 79 us.
+// gradient 38 us; 32768 tokens of 256 experts 36 us, 16384 of 384 41 us, 8192 of
+// 1024 68 us.
 #include "common.cuh"
 
 #include <atomic>
@@ -202,8 +202,8 @@ __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float 
 // takes its place when it is chosen.  Fours of consecutive experts are kept
 // sorted (equal keys in the experts' order, which stands in a word, a byte
 // each), and the largest is that of the fours' heads; of 32, where the order of
-// eight fours costs more than it saves (84 us against 81 for 8192 tokens of 1024
-// experts; of 384: 42 against 52 for 16384), it is looked for again.
+// eight fours costs more than it saves (8192 tokens of 1024 experts: 84 us
+// against 81; 16384 of 384, where it saves: 42 against 52), it is looked for again.
 template <int V>
 struct Keys {
   static constexpr bool kSorted = V <= 16;
@@ -404,21 +404,27 @@ __device__ void first_rows(const Args& a, Sh& sh, int ctas, int cta) {
   add_scan<V>(sh);
 }
 
+// The warp's row of counts: only its own lanes write it before the next barrier.
+template <int V, class Sh>
+__device__ __forceinline__ void zero_counts(Sh& sh) {
+  uint32_t* row = reinterpret_cast<uint32_t*>(sh.cnt[threadIdx.x >> 5]);
+  for (int i = threadIdx.x & 31; i < 16 * V; i += 32) row[i] = 0;
+  __syncwarp();
+}
+
 // Rows of the choices of tokens [t0, t1), a batch of one choice a thread at a
 // time: rank among the batch's earlier choices of the same expert (within the
-// warp by match, over the warps by a column of counts).
+// warp by match, over the warps by a column of counts).  The warps' rows of
+// counts are zero at the call.
 template <int V, class Sh>
 __device__ void assign_rows(const Args& a, Sh& sh, int64_t t0, int64_t t1) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t n0 = t0 * a.k, n1 = t1 * a.k;
-  for (int64_t b = n0; b < n1; b += blockDim.x) {
-    const int64_t left = n1 - b;
+  const int64_t n1 = t1 * a.k;
+  int id = t0 * a.k + threadIdx.x < n1 ? a.ids[t0 * a.k + threadIdx.x] : -1;
+  for (int64_t b = t0 * a.k; b < n1; b += blockDim.x) {
+    const int64_t left = n1 - b, n = b + threadIdx.x;
     const int used = left < blockDim.x ? static_cast<int>((left + 31) / 32) : static_cast<int>(blockDim.x >> 5);
-    uint32_t* zero = reinterpret_cast<uint32_t*>(&sh.cnt[0][0]);
-    for (int i = threadIdx.x; i < used * 16 * V; i += blockDim.x) zero[i] = 0;
-    const int64_t n = b + threadIdx.x;
-    const int id = n < n1 ? a.ids[n] : -1;
-    __syncthreads();
+    const int next = n + blockDim.x < n1 ? a.ids[n + blockDim.x] : -1;
     const uint32_t same = __match_any_sync(FULL, id);
     const int rank = __popc(same & ((1u << lane) - 1u));
     if (id >= 0 && rank == 0) sh.cnt[warp][id] = static_cast<uint16_t>(__popc(same));
@@ -431,12 +437,16 @@ __device__ void assign_rows(const Args& a, Sh& sh, int64_t t0, int64_t t1) {
         sh.cnt[w][e] = static_cast<uint16_t>(run);
         run += c;
       }
-      sh.total[e] = run;
+      const int first = sh.hist[e];  // of the batch; this thread alone goes on with it
+      sh.total[e] = first;
+      sh.hist[e] = first + run;
     }
     __syncthreads();
-    if (n < n1) a.pos[n] = id >= 0 ? sh.hist[id] + sh.cnt[warp][id] + rank : -1;
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += blockDim.x) sh.hist[e] += sh.total[e];
+    if (n < n1) a.pos[n] = id >= 0 ? sh.total[id] + sh.cnt[warp][id] + rank : -1;
+    if (b + blockDim.x >= n1) break;
+    __syncwarp();
+    zero_counts<V>(sh);
+    id = next;
   }
 }
 
@@ -485,6 +495,7 @@ __global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a
   __syncthreads();
   finish<V>(a, sh, a.T < warps<V>() ? static_cast<int>(a.T) : warps<V>(), sh.live);
   add_scan<V>(sh);
+  zero_counts<V>(sh);
   assign_rows<V>(a, sh, 0, a.T);
 }
 
@@ -512,8 +523,11 @@ __global__ void __launch_bounds__(32 * warps<V>(), V <= 4 ? 2 : 1) route_kernel(
 template <int V>
 __global__ void __launch_bounds__(32 * rank_warps<V>()) rank_kernel(const Args a) {
   __shared__ RankShared<V> sh;
-  cudaGridDependencySynchronize();
   const int ctas = gridDim.x - 1, cta = blockIdx.x;
+  const int64_t t0 = static_cast<int64_t>(cta) * a.chunk;
+  const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
+  zero_counts<V>(sh);
+  cudaGridDependencySynchronize();
   first_rows<V>(a, sh, ctas, cta);
   if (cta == ctas) {
     // the CTAs' softmax sums, in as many slices as there are threads for
@@ -534,8 +548,6 @@ __global__ void __launch_bounds__(32 * rank_warps<V>()) rank_kernel(const Args a
     finish<V>(a, sh, slices, n);
     return;
   }
-  const int64_t t0 = static_cast<int64_t>(cta) * a.chunk;
-  const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
   assign_rows<V>(a, sh, t0, t1);
 }
 
