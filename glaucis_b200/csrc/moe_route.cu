@@ -604,8 +604,10 @@ __device__ __forceinline__ void store_token(const Args& a, void* out, int64_t t,
     if (e0 + i < a.E) store_logit(out, a.f32, at + i, v[i]);
 }
 
-// dlogit_e = p_e (c_e + sel_e - sum_e' p_e' (c_e' + sel_e')), c_e = dloss E f_e / n
-// for the loss and sel_e the weights' part on the chosen experts.
+// dlogit_e = p_e (c_e - sum_e' p_e' c_e'), c_e = dloss E f_e / n for the loss; for
+// the gradient d of the chosen experts' weights w plus w_e (d_e - sum_e' w_e' d_e')
+// on those, or, where w is p as it is, p_e d_e there less p_e sum_e' p_e' d_e'
+// everywhere.
 template <int V>
 __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdArgs b) {
   const int lane = threadIdx.x & 31;
@@ -659,12 +661,14 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
     const float inv = softmax<V>(z, zmax, e);
     // the chosen experts' share, in the lane that holds the choice
     const float p_sel = id >= 0 ? exp_of(load_logit(a.logits, a.f32, t * a.E + id) - zmax) * inv : 0.0f;
+    // what the weights add to its logit, and to the sum over the row: none where
+    // the weights are over their sum
+    float add = p_sel * sel, dot = add;
     if (a.renorm) {
-      const float dot = warp_sum(id >= 0 ? sel * w : 0.0f);
-      const float s = warp_sum(p_sel);
-      sel = id >= 0 ? (sel - dot) / s : 0.0f;
+      const float mean = warp_sum(id >= 0 ? sel * w : 0.0f);
+      add = id >= 0 ? w * (sel - mean) : 0.0f;
+      dot = 0.0f;
     }
-    float dot = p_sel * sel;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       e[i] *= inv;
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdA
     // ordered by the warp's barrier)
     if (id >= 0)
       store_logit(b.dlogits, a.f32, t * a.E + id,
-                  p_sel * (static_cast<float>(__ldg(b.counts + id)) * scale + sel - dot));
+                  fmaf(p_sel, static_cast<float>(__ldg(b.counts + id)) * scale - dot, add));
   }
 }
 
