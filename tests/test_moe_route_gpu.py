@@ -79,7 +79,7 @@ def _check_forward(r, ref, logits):
 
 CASES = [(1, 128, 8), (3, 128, 8), (64, 128, 8), (65, 128, 8), (100, 8, 2), (33, 1, 1), (257, 5, 3), (500, 60, 4),
          (129, 160, 6), (300, 256, 8), (2000, 33, 8), (70, 384, 8), (150, 512, 32), (40, 1000, 10), (600, 1024, 32),
-         (10007, 128, 8), (20000, 64, 6)]
+         (10007, 128, 8), (20000, 64, 6), (60, 8, 2), (12, 1000, 2), (9000, 300, 4), (16000, 1000, 8)]
 
 
 @pytest.mark.parametrize("T,E,k", CASES)
