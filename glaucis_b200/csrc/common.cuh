@@ -438,4 +438,43 @@ __device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
   return r;
 }
 
+// A kernel launched with launch_following starts while the one before it in the
+// stream runs out, and waits in follow() until that one is complete and its
+// writes are visible.  Every thread calls follow() before it touches global
+// memory, and nothing is loaded on the read-only path (__ldg), which is not kept
+// coherent with what the other kernel still wrote when this one had started:
+// fetch() instead.  For kernels that follow one another without work of the
+// host's between them: us a call in a stream, against plain launches, one token's
+// 4-bit product 17.4 (18.9), rows out and back with gradients 308 (321).  The
+// norm and the router gained nothing and start plainly.
+// The next kernel launched so may start from the CTAs' call of may_follow() on,
+// by default made at once; it waits in its follow() likewise.
+__device__ __forceinline__ void may_follow() { cudaTriggerProgrammaticLaunchCompletion(); }
+
+__device__ __forceinline__ void follow(bool next = true) {
+  cudaGridDependencySynchronize();
+  if (next) may_follow();
+}
+
+template <class T>
+__device__ __forceinline__ T fetch(const T* p) {
+  return *p;
+}
+
+template <class Kernel, class... Args>
+cudaError_t launch_following(Kernel kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+                             Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace gl

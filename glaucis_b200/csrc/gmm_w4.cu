@@ -34,9 +34,9 @@
 //     exact (values 2^38 below the largest lose bits far under the sum's
 //     rounding), and scaled back where the block's fp32 sum meets the weights'
 //     scale.
-// Measured (K 7168, N 2048, 128 groups): 128 rows in 44 groups 65 us, 5.3 TB/s of
+// Measured (K 7168, N 2048, 128 groups): 128 rows in 44 groups 64 us, 5.4 TB/s of
 // weights and scales (60 us without finishing split jobs, 55 us without the
-// sums); 8 rows in 8 groups 18 us (12 us of loads; the first unit lands 2 us
+// sums); 8 rows in 8 groups 17.4 us (12 us of loads; the first unit lands 2 us
 // after the launch, split jobs are finished 2 us after the last).
 #include "common.cuh"
 
@@ -149,7 +149,7 @@ struct Groups {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int g = g0 + 4 * lane + j;
-      n[j] = g < G ? __ldg(sizes + g) : 0;
+      n[j] = g < G ? fetch(sizes + g) : 0;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -273,7 +273,7 @@ struct XRows {
     for (int i = 0; i < ROWS / 2; ++i) {
       const int r = 2 * i + half;
       v[i] = r < tile.nrows
-                 ? __ldg(a.x + (static_cast<int64_t>(tile.row0 + r) * a.kb + block) * 16 + sub)
+                 ? fetch(a.x + (static_cast<int64_t>(tile.row0 + r) * a.kb + block) * 16 + sub)
                  : make_uint4(0, 0, 0, 0);
     }
   }
@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Abort ab{&ct.abort, a.err};
   Walk walk;
+  follow(false);  // the next kernel starts when the loads are under way, not among them
   if (warp >= WARPS) {
     walk.groups.sizes = a.sizes;
     walk.groups.G = a.G;
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
 
   if (warp == WARPS) {
     // ---- weights and scales, and the stage's control words ----
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // after follow(): their writes, for the copies' proxy
     walk.begin(a, u0);
     int st = 0, n = 0;
     uint32_t phase = 1;  // the first round of stages is free
@@ -464,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
         phase ^= 1;
       }
     }
+    may_follow();
     // the copies land before the CTA may end, also when it gives up
     for (int i = n > S ? n - S : 0; i < n; ++i) {
       const uint64_t from = global_ns();
@@ -706,7 +709,7 @@ int gl_launch_gmm_w4(const void* x, const void* w4, const float* s, const int32_
   const Args a{static_cast<const uint4*>(x), s, group_sizes, tags, parts, next_nonce(), M, N,
                static_cast<int>(G), kb, static_cast<int>(strips), out, out_f32, zero_tail, err};
   if (!gl_set_smem_attr(reinterpret_cast<const void*>(&gmm_w4_kernel), 0, SMEM_BYTES, why)) return -2;
-  gmm_w4_kernel<<<n, THREADS, SMEM_BYTES, st>>>(wmap, a);
+  gl::launch_following(gmm_w4_kernel, n, THREADS, SMEM_BYTES, st, wmap, a);
   return launched(why);
 }
 

@@ -32,7 +32,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // treated as none.
 __device__ __forceinline__ int load_pos(const int* pos, int64_t t, int k, int64_t rows, int* err) {
   const int lane = threadIdx.x & 31;
-  int p = lane < k ? __ldg(pos + t * k + lane) : -1;
+  int p = lane < k ? fetch(pos + t * k + lane) : -1;
   if (p >= rows) {
     atomicExch(err, GL_DEV_BAD_INDEX);
     p = -1;
@@ -54,7 +54,7 @@ __device__ __forceinline__ int64_t first_tail_row(const int* sizes, int G, int64
   long long own = 0;
   bool neg = false;
   for (int g = threadIdx.x; g < G; g += blockDim.x) {
-    const int n = __ldg(sizes + g);
+    const int n = fetch(sizes + g);
     neg = neg || n < 0;
     own += n;
   }
@@ -90,6 +90,7 @@ struct DispatchArgs {
 
 __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a) {
   constexpr int U = 4;
+  follow();
   const int lane = threadIdx.x & 31;
   const int segs = (a.nvec + 32 * U - 1) / (32 * U);
   const int64_t units = a.T * segs, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a) {
     uint4 v[U];
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (v0 + 32 * i < a.nvec) v[i] = __ldg(a.x + t * a.nvec + v0 + 32 * i);
+      if (v0 + 32 * i < a.nvec) v[i] = fetch(a.x + t * a.nvec + v0 + 32 * i);
     const int own = load_pos(a.pos, t, a.k, a.rows, a.err);
     for (int j = 0; j < a.k; ++j) {
       const int64_t p = __shfl_sync(FULL, own, j);
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a) {
       for (int i = 0; i < U; ++i)
         if (v0 + 32 * i < a.nvec) a.out[p * a.nvec + v0 + 32 * i] = v[i];
       if (seg == 0 && a.s)
-        for (int i = lane; i < a.ns; i += 32) a.out_s[p * a.ns + i] = __ldg(a.s + t * a.ns + i);
+        for (int i = lane; i < a.ns; i += 32) a.out_s[p * a.ns + i] = fetch(a.s + t * a.ns + i);
     }
   }
   const int64_t tail = first_tail_row(a.sizes, a.G, a.rows, a.err);
@@ -126,10 +127,10 @@ struct Vec8 {
   uint4 a, b;
   __device__ __forceinline__ void load(const void* y, int64_t vec) {
     if (kF32) {
-      a = __ldg(static_cast<const uint4*>(y) + 2 * vec);
-      b = __ldg(static_cast<const uint4*>(y) + 2 * vec + 1);
+      a = fetch(static_cast<const uint4*>(y) + 2 * vec);
+      b = fetch(static_cast<const uint4*>(y) + 2 * vec + 1);
     } else {
-      a = __ldg(static_cast<const uint4*>(y) + vec);
+      a = fetch(static_cast<const uint4*>(y) + vec);
     }
   }
   __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
@@ -173,6 +174,7 @@ struct CombineArgs {
 // 81, 92 and 81 us (16387 tokens, K 4096).
 template <bool kF32, int B, int U>
 __global__ void __launch_bounds__(256, 4) combine_kernel(const CombineArgs a) {
+  follow();
   const int lane = threadIdx.x & 31;
   const int segs = (a.nvec + 32 * U - 1) / (32 * U);
   const int64_t units = a.T * segs, step = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(256, 4) combine_kernel(const CombineArgs a) {
     const int v0 = static_cast<int>(u - t * segs) * 32 * U + lane;
     const int own = load_pos(a.pos, t, a.k, a.rows, a.err);
     float w_own = own < 0 ? 0.0f : 1.0f;
-    if (a.w && own >= 0) w_own = __ldg(a.w + t * a.k + lane);
+    if (a.w && own >= 0) w_own = fetch(a.w + t * a.k + lane);
     float acc[U][8] = {};
     if (a.res) {
 #pragma unroll
@@ -246,6 +248,7 @@ struct CombineBwdArgs {
 template <int V, bool kF32>
 __global__ void __launch_bounds__(256, V <= 4 ? 4 : 2) combine_bwd_kernel(const CombineBwdArgs a) {
   __shared__ float part[MAX_K][8];
+  follow();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
     float d[V][8];
@@ -258,7 +261,7 @@ __global__ void __launch_bounds__(256, V <= 4 ? 4 : 2) combine_bwd_kernel(const 
       g.floats(d[i]);
     }
     const int own = load_pos(a.pos, t, a.k, a.rows, a.err);
-    const float w_own = own >= 0 ? __ldg(a.w + t * a.k + lane) : 0.0f;
+    const float w_own = own >= 0 ? fetch(a.w + t * a.k + lane) : 0.0f;
     for (int j = 0; j < a.k; ++j) {
       const int64_t p = __shfl_sync(FULL, own, j);
       const float w = __shfl_sync(FULL, w_own, j);
@@ -325,15 +328,15 @@ unsigned warp_ctas(int64_t units, int num_sms) {
 template <bool kF32, int B, int U>
 void combine(const CombineArgs& a, int num_sms, cudaStream_t st) {
   const int64_t units = a.T * ((a.nvec + 32 * U - 1) / (32 * U));
-  combine_kernel<kF32, B, U><<<warp_ctas(units, num_sms), 256, 0, st>>>(a);
+  launch_following(combine_kernel<kF32, B, U>, warp_ctas(units, num_sms), 256, 0, st, a);
 }
 
 template <int V>
 void combine_bwd(const CombineBwdArgs& a, int f32, unsigned ctas, int threads, cudaStream_t st) {
   if (f32)
-    combine_bwd_kernel<V, true><<<ctas, threads, 0, st>>>(a);
+    launch_following(combine_bwd_kernel<V, true>, ctas, threads, 0, st, a);
   else
-    combine_bwd_kernel<V, false><<<ctas, threads, 0, st>>>(a);
+    launch_following(combine_bwd_kernel<V, false>, ctas, threads, 0, st, a);
 }
 
 }  // namespace moe
@@ -349,7 +352,7 @@ int gl_launch_moe_dispatch(const void* x, int64_t row_bytes, const float* s, int
                        static_cast<int>(G), static_cast<int>(row_bytes / 16), static_cast<int>(scales),
                        static_cast<uint4*>(out), out_s, err};
   const int64_t units = T * ((a.nvec + 127) / 128);
-  dispatch_kernel<<<warp_ctas(units, num_sms), 256, 0, st>>>(a);
+  gl::launch_following(dispatch_kernel, warp_ctas(units, num_sms), 256, 0, st, a);
   return launched(why);
 }
 

@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a
 template <int V>
 __global__ void __launch_bounds__(32 * warps<V>(), V <= 4 ? 2 : 1) route_kernel(const Args a) {
   __shared__ RouteShared<V> sh;
-  cudaTriggerProgrammaticLaunchCompletion();
+  may_follow();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.chunk;
   const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
   route_tokens<V>(a, t0, t1, sh);
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(32 * rank_warps<V>()) rank_kernel(const Args a
   const int64_t t0 = static_cast<int64_t>(cta) * a.chunk;
   const int64_t t1 = t0 + a.chunk < a.T ? t0 + a.chunk : a.T;
   zero_counts<V>(sh);
-  cudaGridDependencySynchronize();
+  follow();
   first_rows<V>(a, sh, ctas, cta);
   if (cta == ctas) {
     // the CTAs' softmax sums, in as many slices as there are threads for
@@ -715,17 +715,7 @@ int fwd(const Args& a0, int num_sms, cudaStream_t st, const char** why) {
     route_kernel<V><<<ctas, 32 * warps<V>(), 0, st>>>(a);
     e = cudaGetLastError();
     if (e == cudaSuccess) {
-      // launched while the first runs out; it waits for it on the device
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(ctas + 1);
-      cfg.blockDim = dim3(32 * rank_warps<V>());
-      cfg.stream = st;
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      at[0].val.programmaticStreamSerializationAllowed = 1;
-      cfg.attrs = at;
-      cfg.numAttrs = 1;
-      e = cudaLaunchKernelEx(&cfg, rank_kernel<V>, a);
+      e = launch_following(rank_kernel<V>, ctas + 1, 32 * rank_warps<V>(), 0, st, a);
     }
   }
   if (e == cudaSuccess) return 0;

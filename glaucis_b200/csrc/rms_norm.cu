@@ -317,11 +317,11 @@ __global__ void __launch_bounds__(MAX_T, CTAS) rms_norm_bwd_kernel(const BwdArgs
 __global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float* part, int n, int K, int w32,
                                                            void* dw) {
   __shared__ float sh[32][33];
-  cudaGridDependencySynchronize();
+  follow();
   const int k = blockIdx.x * 32 + (threadIdx.x & 31), rl = threadIdx.x >> 5;
   float s = 0.0f;
   if (k < K)
-    for (int i = rl; i < n; i += 32) s += __ldg(part + static_cast<int64_t>(i) * K + k);
+    for (int i = rl; i < n; i += 32) s += fetch(part + static_cast<int64_t>(i) * K + k);
   sh[rl][threadIdx.x & 31] = s;
   __syncthreads();
   s = warp_sum(sh[threadIdx.x & 31][rl]);
@@ -445,18 +445,9 @@ int gl_launch_rms_norm_bwd(const void* dy, const void* dh, const void* h, const 
       return -2;
     }
   }
-  // launched while the first runs out; it waits for it on the device
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((K + 31) / 32));
-  cfg.blockDim = dim3(1024);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = ctas > 0 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, rms_norm_dw_kernel, static_cast<const float*>(ws), ctas,
-                                           static_cast<int>(K), w32, dw);
+  const cudaError_t e =
+      gl::launch_following(rms_norm_dw_kernel, static_cast<unsigned>((K + 31) / 32), 1024, 0, st,
+                           static_cast<const float*>(ws), ctas, static_cast<int>(K), w32, dw);
   if (e == cudaSuccess) return 0;
   *why = cudaGetErrorString(e);
   return -2;

@@ -228,3 +228,105 @@ def test_calls_on_many_streams(cuda):
         for res in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
     assert ops.device_status() == 0
+
+
+def _buffers(cuda, T, E, k, K):
+    g = torch.Generator(device=cuda).manual_seed(5)
+    r = ops.moe_route_fwd(torch.randn((T, E), generator=g, device=cuda), k)
+    w4, s = ops.quant_w4_128x1(_rand(cuda, E, K, K, seed=6, scale=K ** -0.5))
+    h = _rand(cuda, T, K, seed=7)
+    return dict(r=r, w4=w4, s=s, h=h, h0=h.clone(), xs=torch.empty((T * k, K), dtype=BF16, device=cuda),
+                y=torch.empty((T * k, K), dtype=BF16, device=cuda))
+
+
+@pytest.mark.parametrize("T,E,k,K", [(1, 8, 2, 512), (16, 8, 2, 1024), (300, 16, 2, 2048)])
+def test_each_call_sees_the_one_before(cuda, T, E, k, K):
+    """Calls that read what the call just before them wrote over its own input,
+    one after the other without a pause and in a graph, give what they give with
+    the device idle between them."""
+    b = _buffers(cuda, T, E, k, K)
+    r = b["r"]
+
+    def chain(between):
+        for i in range(12):
+            ops.moe_dispatch_fwd(b["h"], r.pos, r.counts, out=b["xs"])
+            between()
+            ops.gmm_w4_fwd(b["xs"], b["w4"], b["s"], r.counts, out=b["y"])
+            between()
+            ops.moe_combine_fwd(b["y"], r.pos, r.weights, residual=b["h"], out=b["h"])
+            between()
+            if i % 3 == 2:  # else the next dispatch follows at once
+                b["h"].mul_(0.25)
+                between()
+
+    chain(torch.cuda.synchronize)
+    want = b["h"].clone()
+    assert torch.isfinite(want).all()
+    for _ in range(5):
+        b["h"].copy_(b["h0"])
+        chain(lambda: None)
+        assert torch.equal(b["h"], want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b["h"].copy_(b["h0"])
+        chain(lambda: None)
+    for _ in range(5):
+        b["h"].zero_()
+        graph.replay()
+        assert torch.equal(b["h"], want)
+    assert ops.device_status() == 0
+
+
+def test_captured_after_anything(cuda):
+    """A call captured first, after copies, fills, forks and joins of streams."""
+    b = _buffers(cuda, 16, 8, 2, 1024)
+    r, src, other = b["r"], _rand(cuda, 32, 1024, seed=8), torch.cuda.Stream()
+    z, x = torch.zeros(1 << 20, device=cuda), src.clone()
+
+    def call():
+        return ops.gmm_w4_fwd(x, b["w4"], b["s"], r.counts)
+
+    want = call()
+
+    def after_copy():
+        x.copy_(src)
+        return [call()]
+
+    def after_fill():
+        z.zero_()
+        return [call()]
+
+    def after_join():
+        cur = torch.cuda.current_stream()
+        z.add_(1)
+        other.wait_stream(cur)
+        with torch.cuda.stream(other):
+            torch.mul(src, 1, out=x)
+        z.add_(1)
+        cur.wait_stream(other)
+        return [call()]
+
+    def in_a_fork():
+        cur = torch.cuda.current_stream()
+        torch.mul(src, 1, out=x)
+        other.wait_stream(cur)
+        with torch.cuda.stream(other):
+            a = call()
+        c = call()
+        cur.wait_stream(other)
+        return [a, c]
+
+    for step in (lambda: [call()], lambda: [call(), call()], after_copy, after_fill, after_join, in_a_fork):
+        assert all(torch.equal(o, want) for o in step())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for _ in range(5):
+            if step in (after_copy, after_join, in_a_fork):
+                x.zero_()
+            for o in out:
+                o.zero_()
+            graph.replay()
+            assert all(torch.equal(o, want) for o in out)
+        x.copy_(src)
+    assert ops.device_status() == 0
