@@ -445,8 +445,8 @@ __device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
 // coherent with what the other kernel still wrote when this one had started:
 // fetch() instead.  For kernels that follow one another without work of the
 // host's between them: us a call in a stream, against plain launches, one token's
-// 4-bit product 17.4 (18.9), rows out and back with gradients 308 (321).  The
-// norm and the router gained nothing and start plainly.
+// 4-bit product 17.4 (18.9), rows out and back with gradients 308 (321).  Kernels
+// that gained nothing, the norm's backward and the larger routers, start plainly.
 // The next kernel launched so may start from the CTAs' call of may_follow() on,
 // by default made at once; it waits in its follow() likewise.
 __device__ __forceinline__ void may_follow() { cudaTriggerProgrammaticLaunchCompletion(); }

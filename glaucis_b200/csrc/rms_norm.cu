@@ -85,11 +85,11 @@ __device__ __forceinline__ void dot8(const F8& a, const F8& b, float2& acc) {
 template <bool kW32>
 __device__ __forceinline__ F8 load_w8(const void* w, int vec) {
   if (kW32) {
-    const float4 a = __ldg(static_cast<const float4*>(w) + 2 * vec);
-    const float4 b = __ldg(static_cast<const float4*>(w) + 2 * vec + 1);
+    const float4 a = fetch(static_cast<const float4*>(w) + 2 * vec);
+    const float4 b = fetch(static_cast<const float4*>(w) + 2 * vec + 1);
     return {{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
   }
-  return unpack8(__ldg(static_cast<const uint4*>(w) + vec));
+  return unpack8(fetch(static_cast<const uint4*>(w) + vec));
 }
 
 // Sum over the threads of a row: L lanes of a warp, or (L = 0) the CTA's warps
@@ -117,6 +117,7 @@ template <int V, int L, bool kQuant, bool kW32>
 __global__ void __launch_bounds__(L ? SMALL_T : 1024, L == 0 && V == 2 ? 2 : 1) rms_norm_fwd_kernel(const FwdArgs a) {
   constexpr int LL = L ? L : 1;
   __shared__ float part[32];
+  follow();
   const int64_t row = L ? static_cast<int64_t>(blockIdx.x) * (SMALL_T / LL) + threadIdx.x / LL
                         : static_cast<int64_t>(blockIdx.x);
   // rows end inside a warp (two a warp): past them a thread goes on with none
@@ -366,17 +367,17 @@ void launch_fwd(const FwdArgs& a, cudaStream_t st) {
   };
   const unsigned rows = static_cast<unsigned>(a.M);
   if (n <= 16)
-    rms_norm_fwd_kernel<1, 16, kQuant, kW32><<<ctas(16), SMALL_T, 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<1, 16, kQuant, kW32>, ctas(16), SMALL_T, 0, st, a);
   else if (n <= 32)
-    rms_norm_fwd_kernel<1, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<1, 32, kQuant, kW32>, ctas(32), SMALL_T, 0, st, a);
   else if (n <= 64)
-    rms_norm_fwd_kernel<2, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<2, 32, kQuant, kW32>, ctas(32), SMALL_T, 0, st, a);
   else if (n <= 128)
-    rms_norm_fwd_kernel<4, 32, kQuant, kW32><<<ctas(32), SMALL_T, 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<4, 32, kQuant, kW32>, ctas(32), SMALL_T, 0, st, a);
   else if (n <= 1024)
-    rms_norm_fwd_kernel<2, 0, kQuant, kW32><<<rows, row_threads(n, 2), 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<2, 0, kQuant, kW32>, rows, row_threads(n, 2), 0, st, a);
   else  // CTAs of half the threads, more of them an SM: K = 12288 in bf16 59 -> 47 us (5461 rows)
-    rms_norm_fwd_kernel<4, 0, kQuant, kW32><<<rows, row_threads(n, 4), 0, st>>>(a);
+    launch_following(rms_norm_fwd_kernel<4, 0, kQuant, kW32>, rows, row_threads(n, 4), 0, st, a);
 }
 
 // t: threads of a row that a CTA takes.  The shapes are bwd_shape's.
