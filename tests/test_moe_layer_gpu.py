@@ -330,3 +330,44 @@ def test_captured_after_anything(cuda):
             assert all(torch.equal(o, want) for o in out)
         x.copy_(src)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("T,K", [(1, 512), (16, 1024), (300, 1024)])
+def test_norm_and_router_see_the_call_before(cuda, T, K):
+    """The norm reads what the combine just wrote and adds it to the stream in
+    place; the router takes the norm's output as it comes."""
+    E, k = 8, 2
+    b = _buffers(cuda, T, E, k, K)
+    r, w = b["r"], torch.ones(K, dtype=BF16, device=cuda)
+    x, n = b["h0"].clone(), torch.empty_like(b["h0"])
+
+    def chain(between):
+        ids = []
+        x.copy_(b["h0"])
+        b["h"].copy_(b["h0"])
+        for _ in range(8):
+            ops.rms_norm_fwd(x, w, residual=b["h"], y=n, h=b["h"])
+            between()
+            ids.append(ops.moe_route_fwd(n, 4).ids)
+            between()
+            ops.moe_dispatch_fwd(n, r.pos, r.counts, out=b["xs"])
+            between()
+            ops.gmm_w4_fwd(b["xs"], b["w4"], b["s"], r.counts, out=b["y"])
+            between()
+            ops.moe_combine_fwd(b["y"], r.pos, r.weights, out=x)
+            between()
+        return torch.stack(ids)
+
+    ids = chain(torch.cuda.synchronize)
+    want = b["h"].clone()
+    assert torch.isfinite(want).all()
+    for _ in range(5):
+        assert torch.equal(chain(lambda: None), ids) and torch.equal(b["h"], want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(lambda: None)
+    for _ in range(5):
+        b["h"].zero_()
+        graph.replay()
+        assert torch.equal(got, ids) and torch.equal(b["h"], want)
+    assert ops.device_status() == 0
