@@ -609,6 +609,7 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
   if (own_split) there = static_cast<int>(atom_add_acq_rel(own_tag, 1) & 0xFFFF);
   const bool complete = own_split && there == static_cast<int>(own_to - own_from);
   if (complete) *own_tag = 0;
+  __syncwarp();  // what the counting lane acquired, for the lanes that read the parts
 #pragma unroll
   for (int l = 0; l < 2; ++l) {
     if (!__shfl_sync(FULL, complete, l)) continue;

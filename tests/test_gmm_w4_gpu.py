@@ -203,6 +203,22 @@ def test_graph_replays_share_nothing(cuda):
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+@pytest.mark.parametrize("K,N,sizes", [(14336, 512, [1]), (7168, 512, [8]), (7168, 1024, [3, 0, 2, 5])])
+def test_jobs_of_many_ctas_are_the_same_every_time(cuda, K, N, sizes):
+    # every tile's k is cut among CTAs, and whichever of them is last adds all parts
+    w4, s = _weights(cuda, len(sizes), K, N, seed=13)
+    x = _x(cuda, sum(sizes), K, seed=14)
+    gs = torch.tensor(sizes, dtype=torch.int32, device=cuda)
+    first = ops.gmm_w4_fwd(x, w4, s, gs)
+    _check(first, x, w4, s, sizes, K)
+    busy = torch.empty(1 << 27, dtype=torch.uint8, device=cuda)
+    for i in range(100):
+        if i % 2:
+            busy.fill_(i)  # the parts leave the caches, the CTAs start at other times
+        assert torch.equal(ops.gmm_w4_fwd(x, w4, s, gs), first)
+    assert ops.device_status() == 0
+
+
 def test_refusals(cuda):
     w4, s = _weights(cuda, 2, 256, 64)
     x, gs = _x(cuda, 4, 256), torch.tensor([2, 2], dtype=torch.int32, device=cuda)
