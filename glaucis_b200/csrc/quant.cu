@@ -30,48 +30,10 @@
 
 namespace gl {
 
-// Division by a block scale.  With y = RN(1/s) (one IEEE division per
-// block), q = RN(x*y) lies within one ulp of x/s, the residual r = x - q*s is
-// exact in one FMA, and RN(q + r*y) is the correctly rounded quotient
-// (P. Markstein, "Computation of elementary functions on the IBM RISC
-// System/6000 processor", IBM J. Res. Develop. 34(1), 1990).  The residual is
-// exact only while it stays above the subnormal range: with s >= 2^-64 every
-// element whose quotient can reach a non-zero e4m3 value has |x| >= 2^-74, far
-// from it.  Blocks with smaller (or non-finite) scales take the plain
-// division.  A quotient by s > 0 has the sign of x; the packed form
-// (markstein2) works on -x and -y so that x = -0 keeps its sign without a
-// copysign.  The arithmetic runs on packed f32x2 FMAs.  Tests compare this
-// path with IEEE division for every finite bf16 block maximum and every bf16
-// element value.
-struct BlockDiv {
-  float s, y;
-  bool fast;
-  BlockDiv() = default;
-  __device__ __forceinline__ explicit BlockDiv(float scale) : s(scale) {
-    fast = scale >= 0x1p-64f && scale <= 3.40282347e38f;
-    y = 1.0f / scale;
-  }
-  // recip = 1.0f / scale computed elsewhere (the same IEEE division)
-  __device__ __forceinline__ BlockDiv(float scale, float recip) : s(scale), y(recip) {
-    fast = scale >= 0x1p-64f && scale <= 3.40282347e38f;
-  }
-};
-
 // The two bf16 values of w as negated floats (sign bit flipped in the same
 // integer operation that widens them).
 __device__ __forceinline__ float2 bf16x2_to_neg_f32x2(uint32_t w) {
   return make_float2(__uint_as_float((w << 16) ^ 0x80000000u), __uint_as_float((w & 0xFFFF0000u) ^ 0x80000000u));
-}
-
-// Markstein's quotient of two elements on packed FMAs, in negated form so
-// that zeros keep their sign without a copysign: with nx = -x and ny = -y,
-// q = nx ny = RN(x y), r' = RN(q s + nx) = q s - x (exact, = -r),
-// v = RN(r' ny + q) = RN(q + r y).  For x = +0: q = +0, r' = +0,
-// v = -0 + +0 = +0; for x = -0: q = -0, r' = +0, v = -0 + -0 = -0.
-__device__ __forceinline__ float2 markstein2(float2 nx, float2 ny, float2 s) {
-  const float2 q = __fmul2_rn(nx, ny);
-  const float2 r = __ffma2_rn(q, s, nx);
-  return __ffma2_rn(r, ny, q);
 }
 
 // Eight bf16 values (one 16-byte chunk) -> eight e4m3 bytes.

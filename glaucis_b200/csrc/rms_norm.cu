@@ -13,7 +13,7 @@
 // Both passes are bound by HBM: a row is read once, held in registers as
 // 16-byte vectors (8 features a thread and vector) and written once.  The row
 // sums are held in 32 bits and reduced in a fixed order.  Of 64 Mi elements the
-// 8-bit output with residual takes 0.88 to 1.02 of the copy rate from 128 to
+// 8-bit output with residual takes 0.86 to 1.02 of the copy rate from 128 to
 // 16384 features, the backward 0.82 to 1.09, the bf16 output alone 0.81 to 1.0.
 #include "common.cuh"
 
@@ -58,6 +58,13 @@ __device__ __forceinline__ F8 unpack8(const uint4& u) {
 __device__ __forceinline__ uint4 pack8(const F8& f) {
   return make_uint4(pack_bf16x2(f.p[0].x, f.p[0].y), pack_bf16x2(f.p[1].x, f.p[1].y),
                     pack_bf16x2(f.p[2].x, f.p[2].y), pack_bf16x2(f.p[3].x, f.p[3].y));
+}
+
+__device__ __forceinline__ F8 neg8(const F8& a) {
+  F8 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.p[j] = make_float2(-a.p[j].x, -a.p[j].y);
+  return r;
 }
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
@@ -159,10 +166,11 @@ __global__ void __launch_bounds__(L ? SMALL_T : 1024, L == 0 && V == 2 ? 2 : 1) 
   for (int i = 0; i < V; ++i) {
     const int vec = tid + i * step;
     const bool in = vec < nvec;
-    F8 f = scale8(unpack8(xv[i]), r);
+    // y, or with the 8-bit output -y, as its division takes it (markstein2)
+    F8 f = scale8(unpack8(xv[i]), kQuant ? -r : r);
     if (in) {  // past the row all are 0
       f = mul8(f, load_w8<kW32>(a.w, vec));
-      if (a.y) a.y[base + vec] = pack8(f);
+      if (a.y) a.y[base + vec] = pack8(kQuant ? neg8(f) : f);
     }
     if (kQuant) {
       // a block of 128 features is a half-warp's vectors (nvec % 16 == 0, so
@@ -173,17 +181,20 @@ __global__ void __launch_bounds__(L ? SMALL_T : 1024, L == 0 && V == 2 ? 2 : 1) 
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
       float s;
-      if (m == 0.0f || (m >= 0x1p-90f && m <= 3.40282347e38f)) {
+      if (m == 0.0f || (m >= 0x1p-55f && m <= 3.40282347e38f)) {
         // m / 448 correctly rounded (Markstein: the rounded product with the
-        // rounded reciprocal, then one correction), its reciprocal to 1 ulp
+        // rounded reciprocal, then one correction), then the elements' quotients
+        // likewise: the scale stays above BlockDiv's bound
         constexpr float R = 1.0f / 448.0f;
         s = m * R;
         s = m == 0.0f ? 1.0f : fmaf(fmaf(-s, 448.0f, m), R, s);
-        f = scale8(f, __fdividef(1.0f, s));
+        const float2 ny = both(-__frcp_rn(s)), s2 = both(s);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.p[j] = markstein2(f.p[j], ny, s2);
       } else {  // tiny or infinite: each element divided
         s = m / 448.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f.p[j] = make_float2(f.p[j].x / s, f.p[j].y / s);
+        for (int j = 0; j < 4; ++j) f.p[j] = make_float2(-f.p[j].x / s, -f.p[j].y / s);
       }
       if (in) {
         uint32_t p[4];

@@ -161,6 +161,24 @@ def test_tiny_outputs_divide(cuda):
     _check_pair(q, s, _norm64(x, w)[0], K)
 
 
+@pytest.mark.parametrize("M,K", [(64, 128), (9, 256), (33, 1024), (3, 2048), (40, 7168), (2, 16384)])
+@pytest.mark.parametrize("residual,w32", [(False, True), (True, False), (True, True)])
+def test_pair_is_the_rounded_quotient(cuda, M, K, residual, w32):
+    # y as the kernel has it, in 32 bits: two rounded products with its own rstd.
+    # From there the pair is the activation quantiser's, byte for byte: the scale
+    # a correctly rounded quotient and q = e4m3(y / s) of another one.
+    x, res, w, _, _ = _inputs(cuda, M, K, residual, w32, seed=12)
+    x[0, ::5], w[3::7] = -0.0, 0.0
+    f = ops.rms_norm_fwd(x, w, EPS, residual=res, output_quant=True)
+    y = (f.h.float() * f.rstd[:, None]) * w.float()
+    b = y.reshape(M, K // 128, 128)
+    s = (b.abs().amax(2).double() / 448).float()
+    s = torch.where(s == 0, 1.0, s)
+    assert torch.equal(f.s, s)
+    q = (b.double() / s.double()[:, :, None]).float().to(torch.float8_e4m3fn).reshape(M, K)
+    assert torch.equal(f.q.view(torch.uint8), q.view(torch.uint8))
+
+
 def test_sum_may_replace_an_input(cuda):
     x, res, w, _, _ = _inputs(cuda, 50, 2048, True, False, seed=7)
     q, s, h = ops.rms_norm_quant_1x128(x, w, residual=res)
