@@ -78,7 +78,7 @@ __device__ __forceinline__ void zero_rows(uint4* out, int nvec, int64_t first, i
 
 struct DispatchArgs {
   const uint4* x;
-  const float* s;      // or null
+  const float* s;      // null without scales (ns 0) or tokens
   const int* pos;
   const int* sizes;
   int64_t T, rows;
@@ -109,13 +109,13 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const DispatchArgs a) {
 #pragma unroll
       for (int i = 0; i < U; ++i)
         if (v0 + 32 * i < a.nvec) a.out[p * a.nvec + v0 + 32 * i] = v[i];
-      if (seg == 0 && a.s)
+      if (seg == 0)
         for (int i = lane; i < a.ns; i += 32) a.out_s[p * a.ns + i] = fetch(a.s + t * a.ns + i);
     }
   }
   const int64_t tail = first_tail_row(a.sizes, a.G, a.rows, a.err);
   zero_rows(a.out, a.nvec, tail, a.rows);
-  if (a.s)
+  if (a.ns)  // also without tokens, where s has no address
     for (int64_t i = tail * a.ns + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
          i < a.rows * a.ns; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
       a.out_s[i] = 1.0f;

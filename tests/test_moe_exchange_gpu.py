@@ -201,6 +201,23 @@ def test_bad_rows_and_sizes_are_reported(cuda):
         assert torch.equal(out, x.repeat_interleave(2, 0))
 
 
+def test_no_tokens_but_rows_of_a_capacity(cuda):
+    K, rows, k = 256, 40, 2
+    pos = torch.empty((0, k), dtype=torch.int32, device=cuda)
+    sizes = torch.zeros(4, dtype=torch.int32, device=cuda)
+    q = torch.empty((0, K), dtype=torch.float8_e4m3fn, device=cuda)
+    s = torch.empty((0, K // 128), device=cuda)
+    out = torch.full((rows, K), float("nan"), device=cuda).to(torch.float8_e4m3fn)
+    out_s = torch.full((rows, K // 128), float("nan"), device=cuda)
+    ops.moe_dispatch_quant(q, s, pos, sizes, rows, out=out, out_s=out_s)
+    assert (out.float() == 0).all() and (out_s == 1).all()
+    y = torch.ones((rows, K), device=cuda)
+    dy, dw = ops.moe_combine_bwd(torch.empty((0, K), dtype=torch.bfloat16, device=cuda), y, pos,
+                                 torch.empty((0, k), device=cuda), sizes)
+    assert (dy == 0).all() and dw.shape == (0, k)
+    assert ops.device_status() == 0
+
+
 def test_refusals(cuda):
     T, K = 4, 256
     x, pos = _rand(cuda, T, K), torch.zeros((T, 2), dtype=torch.int32, device=cuda)
