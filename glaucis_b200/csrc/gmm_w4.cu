@@ -10,37 +10,31 @@
 // what a call does before its first load.
 //   * One launch.  A persistent CTA takes an equal share of all (tile of 8
 //     rows, 512 columns, 128 k) units, cut at any k, so no SM waits for another
-//     one's longer list.  One thread copies weights and scales of the units
-//     into a ring of shared-memory stages with TMA, running ahead across
-//     tiles; a warp per stage puts the rows of x beside them in fragment order
-//     (one warp for all of them held the product back); eight warps take 64
-//     columns each (with 32, what a unit costs besides its weights did).
+//     one's longer list.  One thread copies weights, scales and rows of x of the
+//     units into a ring of shared-memory stages with TMA, running ahead across
+//     tiles; eight warps take 64 columns each (with 32, what a unit costs besides
+//     its weights held the product back).
 //   * Where a share ends inside a tile's k, its fp32 sums go to the workspace;
 //     when its share is done a warp counts its parts in, and whoever completes a
 //     job's count adds the parts in order: the result does not depend on which
 //     one that is, and nothing waits.  (Counting in at the job's end, amid the
 //     loads, stood in their queue: 6 us of 20 for one token.)
-//   * Weights go through mma.sync (m16n8k16, fp16 in, fp32 sums) as the 16-row
+//   * Weights go through mma.sync (m16n8k16, bf16 in, fp32 sums) as the 16-row
 //     operand, 8 rows of x as the 8 columns: enough rate for a memory-bound
 //     product.  (A tcgen05 tile would need the weights widened and written back
 //     to shared memory first, and has 128 rows.)
-//   * A nibble is used as it lies in the word: masked, it is the fp16
-//     subnormal u * 2^-24 (or 16 u * 2^-24 four bits up), exact in the matrix
-//     unit.  Eight weights cost four ANDs and one shift.  The x that meets the
-//     second nibble of a byte is stored divided by 16, and the offset 8 * sum(x)
-//     starts the sum with its negative.
-//   * x is bf16, whose range fp16 lacks: every 128-block of a row is scaled by
-//     a power of two that takes its largest value to [2^13, 2^14), which is
-//     exact (values 2^38 below the largest lose bits far under the sum's
-//     rounding), and scaled back where the block's fp32 sum meets the weights'
-//     scale.
-// Measured (K 7168, N 2048, 128 groups): 128 rows in 44 groups 64 us, 5.4 TB/s of
-// weights and scales (60 us without finishing split jobs, 55 us without the
-// sums); 8 rows in 8 groups 17.4 us (12 us of loads; the first unit lands 2 us
-// after the launch, split jobs are finished 2 us after the last).
+//   * Both operands are exact: x as it was given, and q 2^-6 as a bf16 number,
+//     which costs a masked nibble one packed FMA (eight weights: four ANDs, one
+//     shift, four FMAs).  Left as they are, u = q + 8, the nibbles would cost no
+//     FMA, with 8 sum(x) taken off the sum (one token 16.7 us for 17.9, 128 rows
+//     62 for 67); but then an x whose weight is 0 leaves the rounding of 8 x
+//     behind: with an outlier of 1e4 among x of unit size errors of 1e-2 in place
+//     of 1e-6.
+// Sums stay in fp32's range while those of |q x| in a block stay below 2^134.
+// Measured in a CUDA graph (K 7168, N 2048, 128 groups): 128 rows in 44 groups 67
+// us, 5.2 TB/s of weights and scales (64 us without finishing split jobs, 54.5 us
+// without the sums too); 8 rows in 8 groups 17.9 us (15.7, 11.9).
 #include "common.cuh"
-
-#include <cuda_fp16.h>
 
 #include <atomic>
 
@@ -54,23 +48,22 @@ constexpr int ROWS = 8;            // rows of a tile
 constexpr int COLS = 512;          // columns of a unit: 64 for each of the
 constexpr int WARPS = COLS / 64;   // consumer warps
 constexpr int STAGES = 3;          // two CTAs an SM
-constexpr int THREADS = 32 * (WARPS + 1 + STAGES);
+constexpr int THREADS = 32 * (WARPS + 1);
 constexpr int MIN_UNITS = 2;       // a share is no smaller: a part's way through the workspace costs more
-// A stage: the weights as TMA leaves them, 32-column strips of 16 words a
-// column, 128-byte rows swizzled (16-byte chunk c of row r at c ^ (r & 7)); the
-// scales; the rows of x, 128 fp16 each (every 8 in the order 0 4 1 5 2 6 3 7,
-// odd ones / 16), then two floats (-8 * 2^-24 * sum of the scaled x, 2^(e + 12)).
-// In a 16-byte access phase lanes (gq, t), two gq and four t, read words 2 t +
-// const of the weights: chunks gq ^ (2 t + const) are eight different bank
-// groups, and so are rows of x 272 bytes apart.
+// A stage as TMA leaves it: the weights, 32-column strips of 16 words a column;
+// the scales; the rows of x, 64 features each, twice.  The 128-byte rows of
+// weights and x are swizzled (16-byte chunk c of row r at c ^ (r & 7)).  In a
+// 16-byte access phase lanes (gq, t), two gq and four t, read words 2 t + const
+// of the weights: chunks gq ^ (2 t + const) are eight different bank groups; and
+// of row gq of x the chunks 2 t + const, as many.
 constexpr int S_OFF = COLS * 64;
 constexpr int X_OFF = S_OFF + COLS * 4;
-constexpr int X_BYTES = 272;
-constexpr int STAGE_BYTES = (X_OFF + ROWS * X_BYTES + 1023) / 1024 * 1024;
+constexpr int X_BYTES = ROWS * 256;
+constexpr int STAGE_BYTES = X_OFF + X_BYTES;
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024;  // aligned to 1 KB inside
+static_assert(X_OFF % 1024 == 0 && STAGE_BYTES % 1024 == 0, "swizzled rows start at 1 KB");
 
 struct Args {
-  const uint4* x;
   const float* s;      // [G, K / 128, N]
   const int* sizes;
   unsigned long long* tags;  // [CTAs, WARPS]: the call's number << 16, plus parts that are there
@@ -86,20 +79,27 @@ struct Args {
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                     uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The same with its own third operand.
-__device__ __forceinline__ void mma(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                    uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// q 2^-6 of the nibbles 0 and 4 (lo) or 1 and 5 (hi) of a word, exact: a masked
+// nibble u is the bf16 number u 2^-133, or 16 u 2^-133 four bits up (the step
+// from the subnormals to the first normal ones, at u = 8, keeps the spacing).
+__device__ __forceinline__ uint32_t weights_lo(uint32_t w) {
+  return fma_bf16x2(w & 0x000F000Fu, 0x7F007F00u /* 2^127 */, 0xBE00BE00u /* -8 * 2^-6 */);
+}
+
+__device__ __forceinline__ uint32_t weights_hi(uint32_t w) {
+  return fma_bf16x2(w & 0x00F000F0u, 0x7D007D00u /* 2^123 */, 0xBE00BE00u);
 }
 
 __device__ __forceinline__ uint4 lds4(uint32_t addr) {
@@ -113,12 +113,6 @@ __device__ __forceinline__ uint4 lds4(uint32_t addr) {
 __device__ __forceinline__ float4 lds4f(uint32_t addr) {
   const uint4 v = lds4(addr);
   return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-}
-
-__device__ __forceinline__ float2 lds2f(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
-  return v;
 }
 
 __device__ __forceinline__ unsigned long long atom_add_acq_rel(unsigned long long* p, unsigned long long v) {
@@ -259,67 +253,8 @@ struct Control {
   int4 job[STAGES];  // then: the job, the tile's first row, its strip
   int4 part[2];      // row0, nrows, strip of the first and the last job, where the CTA has a part only
   Shares shares;
+  int tail;          // first row to be zeroed
   int abort;
-};
-
-// The rows of x of one unit on their way to shared memory: half a warp a row,
-// eight features a lane.
-struct XRows {
-  uint4 v[ROWS / 2];
-
-  __device__ __forceinline__ void load(const Args& a, const Tile& tile, int block) {
-    const int half = (threadIdx.x >> 4) & 1, sub = threadIdx.x & 15;
-#pragma unroll
-    for (int i = 0; i < ROWS / 2; ++i) {
-      const int r = 2 * i + half;
-      v[i] = r < tile.nrows
-                 ? fetch(a.x + (static_cast<int64_t>(tile.row0 + r) * a.kb + block) * 16 + sub)
-                 : make_uint4(0, 0, 0, 0);
-    }
-  }
-
-  __device__ __forceinline__ void store(uint32_t at, int nrows) const {
-    const int half = (threadIdx.x >> 4) & 1, sub = threadIdx.x & 15;
-#pragma unroll
-    for (int i = 0; i < ROWS / 2; ++i) {
-      if (2 * i < nrows) {
-        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        float f[8], m = 0.0f, sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 p = bf16x2_to_f32x2(w[j]);
-          f[2 * j] = p.x;
-          f[2 * j + 1] = p.y;
-          m = fmaxf(m, fmaxf(fabsf(p.x), fabsf(p.y)));
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-        // exponent of the largest value, to 2^13; blocks below 2^-113 take 2^126
-        int e = static_cast<int>(__float_as_uint(m) >> 23) - 127 - 13;
-        e = e < -126 ? -126 : e;
-        const float scale = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[j] *= scale;
-          sum += f[j];
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float d = j & 1 ? 0.0625f : 1.0f;
-          const __half2 p = __floats2half2_rn(f[j] * d, f[j + 4] * d);
-          h[j] = *reinterpret_cast<const uint32_t*>(&p);
-        }
-        const uint32_t row = at + (2 * i + half) * X_BYTES;
-        st_shared_v4(row + sub * 16, h[0], h[1], h[2], h[3]);
-        if (sub == 0)
-          st_shared_v4(row + 256, __float_as_uint(sum * -0x1p-21f), static_cast<uint32_t>(127 + e + 12) << 23, 0,
-                       0);
-      }
-    }
-  }
 };
 
 // The lane's sums as four pieces of four columns: piece e is row 2 t + (e & 1)
@@ -391,6 +326,7 @@ __device__ __forceinline__ void add_parts(const Args& a, const int4& job, uint32
 }
 
 __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constant__ CUtensorMap wmap,
+                                                            const __grid_constant__ CUtensorMap xmap,
                                                             const Args a) {
   constexpr int S = STAGES;
   extern __shared__ char smem_raw[];
@@ -400,46 +336,46 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
   const Abort ab{&ct.abort, a.err};
   Walk walk;
   follow(false);  // the next kernel starts when the loads are under way, not among them
-  if (warp >= WARPS) {
+  if (warp == WARPS) {
     walk.groups.sizes = a.sizes;
     walk.groups.G = a.G;
     walk.groups.M = static_cast<int>(a.M);
     int total = 0;
     const int tiles = walk.groups.count(total);
-    if (warp == WARPS) {
-      if (lane == 0) {
-        prefetch_tmap(&wmap);
-        ct.abort = 0;
-        const uint32_t units = tiles < 0 ? 0 : static_cast<uint32_t>(tiles) * a.strips * a.kb;
-        const uint32_t most = (units + MIN_UNITS - 1) / MIN_UNITS;
-        Shares sh;
-        sh.ctas = most < gridDim.x ? most : gridDim.x;
-        sh.each = sh.ctas ? units / sh.ctas : 0;
-        sh.longer = sh.ctas ? units - sh.each * sh.ctas : 0;
-        ct.shares = sh;
-        for (int i = 0; i < S; ++i) {
-          mbar_init(&ct.full[i], 2);
-          mbar_init(&ct.empty[i], WARPS);
-        }
-        fence_mbar_init();
+    if (lane == 0) {
+      prefetch_tmap(&wmap);
+      prefetch_tmap(&xmap);
+      ct.abort = 0;
+      ct.tail = tiles < 0 ? static_cast<int>(a.M) : total;
+      if (tiles < 0 && blockIdx.x == 0) atomicExch(a.err, GL_DEV_BAD_GROUPS);
+      const uint32_t units = tiles < 0 ? 0 : static_cast<uint32_t>(tiles) * a.strips * a.kb;
+      const uint32_t most = (units + MIN_UNITS - 1) / MIN_UNITS;
+      Shares sh;
+      sh.ctas = most < gridDim.x ? most : gridDim.x;
+      sh.each = sh.ctas ? units / sh.ctas : 0;
+      sh.longer = sh.ctas ? units - sh.each * sh.ctas : 0;
+      ct.shares = sh;
+      for (int i = 0; i < S; ++i) {
+        mbar_init(&ct.full[i], 1);
+        mbar_init(&ct.empty[i], WARPS);
       }
-    } else if (tiles < 0) {
-      if (blockIdx.x == 0 && lane == 0) atomicExch(a.err, GL_DEV_BAD_GROUPS);
-    } else if (a.zero_tail && warp == WARPS + 1) {
-      const int64_t words = a.N * (a.out_f32 ? 4 : 2) / 16;
-      for (int64_t i = total * words + static_cast<int64_t>(blockIdx.x) * 32 + lane; i < a.M * words;
-           i += static_cast<int64_t>(gridDim.x) * 32)
-        static_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+      fence_mbar_init();
     }
   }
   __syncthreads();
+  if (a.zero_tail && warp < WARPS) {  // while the first loads are under way
+    const int64_t words = a.N * (a.out_f32 ? 4 : 2) / 16;
+    for (int64_t i = ct.tail * words + static_cast<int64_t>(blockIdx.x) * (32 * WARPS) + threadIdx.x; i < a.M * words;
+         i += static_cast<int64_t>(gridDim.x) * (32 * WARPS))
+      static_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+  }
   const Shares sh = ct.shares;
   if (blockIdx.x >= sh.ctas) return;
   const uint32_t u0 = sh.start(blockIdx.x);
   const int units = static_cast<int>(sh.start(blockIdx.x + 1) - u0);
 
   if (warp == WARPS) {
-    // ---- weights and scales, and the stage's control words ----
+    // ---- weights, scales and rows of x, and the stage's control words ----
     asm volatile("fence.proxy.async.global;" ::: "memory");  // after follow(): their writes, for the copies' proxy
     walk.begin(a, u0);
     int st = 0, n = 0;
@@ -453,12 +389,14 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
         const bool ends = walk.block == a.kb - 1 || n == units - 1;
         ct.rows[st] = ends ? -tile.nrows : tile.nrows;
         if (ends) ct.job[st] = make_int4(walk.job, tile.row0, walk.strip, 0);
-        mbar_arrive_expect_tx(&ct.full[st], S_OFF + bytes);
+        mbar_arrive_expect_tx(&ct.full[st], S_OFF + bytes + X_BYTES);
         char* dst = smem_raw + (smem - smem_u32(smem_raw)) + st * STAGE_BYTES;
         const int64_t kb = static_cast<int64_t>(tile.group) * a.kb + walk.block;
         // columns past N are filled with zeros and counted
         tma_load_3d(dst, &wmap, &ct.full[st], 0, static_cast<int>(kb * 16), walk.strip * (COLS / 32));
         bulk_load(dst + S_OFF, a.s + kb * a.N + n0, bytes, &ct.full[st]);
+        // always 8 rows: those past the tile's are other rows of x, or zeros
+        tma_load_3d(dst + X_OFF, &xmap, &ct.full[st], 0, tile.row0, 2 * walk.block);
       }
       walk.advance(a, n + 1 < units);
       if (++st == S) {
@@ -476,33 +414,12 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
     return;
   }
 
-  if (warp > WARPS) {
-    // ---- rows of x: a warp takes the units of one stage; a unit's rows are on
-    // their way while the stage is still in use ----
-    const int st = warp - WARPS - 1;
-    if (st >= units) return;
-    walk.begin(a, u0);
-    for (int i = 0; i < st; ++i) walk.advance(a, true);
-    uint32_t phase = 1;  // the first round is free
-    for (int n = st; n < units; n += S) {
-      XRows rows;
-      rows.load(a, walk.tile, walk.block);
-      if (n >= S && !mbar_wait(&ct.empty[st], phase, ab)) return;
-      rows.store(smem + st * STAGE_BYTES + X_OFF, walk.tile.nrows);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ct.full[st]);
-      phase ^= 1;
-      for (int i = 1; i <= S; ++i) walk.advance(a, n + S < units);
-    }
-    return;
-  }
-
   // ---- consumers: 64 columns a warp; lane (gq, t) holds columns 4 gq .. 4 gq
   // + 3 of each half and four of the words k / 8 ----
   const int gq = lane >> 2, t = lane & 3;
   const uint32_t w_even = warp * 4096 + sw128_off(2 * t, gq), w_odd = warp * 4096 + sw128_off(2 * t + 1, gq);
-  const uint32_t s_at = S_OFF + warp * 256 + gq * 16, x_at = X_OFF + gq * X_BYTES + t * 32;
-  const uint32_t xs_at = X_OFF + 2 * t * X_BYTES + 256;
+  const uint32_t s_at = S_OFF + warp * 256 + gq * 16;
+  const uint32_t x_even = X_OFF + sw128_off(gq, 2 * t), x_odd = X_OFF + sw128_off(gq, 2 * t + 1);
   // The jobs of which this CTA may have a part only, its first (lane 0) and its
   // last (lane 1), and the counts of their parts.  A count is taken over for
   // this call by whoever comes first; each of a job's CTAs looks before it adds
@@ -539,41 +456,37 @@ __global__ void __launch_bounds__(THREADS, 2) gmm_w4_kernel(const __grid_constan
       w[h][3] = lds4(p + w_odd + h * 2048 + 1024);
     }
     const float4 s0 = lds4f(p + s_at), s1 = lds4f(p + s_at + 128);
-    // 2^24 of the nibbles and 2^e of x, 12 of them on the scale: neither
-    // product leaves fp32's range before the other factor brings it back
-    const float sc[8] = {s0.x * 4096.0f, s0.y * 4096.0f, s0.z * 4096.0f, s0.w * 4096.0f,
-                         s1.x * 4096.0f, s1.y * 4096.0f, s1.z * 4096.0f, s1.w * 4096.0f};
-    // Rows past the tile's hold what an earlier unit left: a column of the
-    // matrix unit's result depends on its own row of x alone, and theirs are
-    // not stored.
-    const uint4 x[4] = {lds4(p + x_at), lds4(p + x_at + 16), lds4(p + x_at + 128), lds4(p + x_at + 144)};
-    const float2 xs0 = lds2f(p + xs_at), xs1 = lds2f(p + xs_at + X_BYTES);
-    const float offset[4] = {xs0.x, xs1.x, xs0.x, xs1.x};
-    float acc[4][4];
+    // 2^6 of the weights
+    const float sc[8] = {s0.x * 64.0f, s0.y * 64.0f, s0.z * 64.0f, s0.w * 64.0f,
+                         s1.x * 64.0f, s1.y * 64.0f, s1.z * 64.0f, s1.w * 64.0f};
+    // Rows past the tile's: a column of the matrix unit's result depends on its
+    // own row of x alone, and theirs are not stored.
+    const uint4 x[4] = {lds4(p + x_even), lds4(p + x_odd), lds4(p + x_even + 1024), lds4(p + x_odd + 1024)};
+    float acc[4][4] = {};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t c[8] = {w[0][i].x, w[0][i].y, w[0][i].z, w[0][i].w,
                              w[1][i].x, w[1][i].y, w[1][i].z, w[1][i].w};
+      // the features in the nibbles' order: 0 4, 1 5, 2 6, 3 7
+      const uint32_t b0 = __byte_perm(x[i].x, x[i].z, 0x5410), b1 = __byte_perm(x[i].x, x[i].z, 0x7632);
+      const uint32_t b2 = __byte_perm(x[i].y, x[i].w, 0x5410), b3 = __byte_perm(x[i].y, x[i].w, 0x7632);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const uint32_t l = c[2 * h], v = c[2 * h + 1];
-        if (i == 0)
-          mma(acc[h], offset, l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[0].x, x[0].y);
-        else
-          mma(acc[h], l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[i].x, x[i].y);
+        mma(acc[h], weights_lo(l), weights_lo(v), weights_hi(l), weights_hi(v), b0, b1);
       }
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const uint32_t l = c[2 * h] >> 8, v = c[2 * h + 1] >> 8;
-        mma(acc[h], l & 0x000F000Fu, v & 0x000F000Fu, l & 0x00F000F0u, v & 0x00F000F0u, x[i].z, x[i].w);
+        mma(acc[h], weights_lo(l), weights_lo(v), weights_hi(l), weights_hi(v), b2, b3);
       }
     }
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      tot[h][0] = fmaf(acc[h][0] * sc[2 * h], xs0.y, tot[h][0]);
-      tot[h][1] = fmaf(acc[h][1] * sc[2 * h], xs1.y, tot[h][1]);
-      tot[h][2] = fmaf(acc[h][2] * sc[2 * h + 1], xs0.y, tot[h][2]);
-      tot[h][3] = fmaf(acc[h][3] * sc[2 * h + 1], xs1.y, tot[h][3]);
+      tot[h][0] = fmaf(acc[h][0], sc[2 * h], tot[h][0]);
+      tot[h][1] = fmaf(acc[h][1], sc[2 * h], tot[h][1]);
+      tot[h][2] = fmaf(acc[h][2], sc[2 * h + 1], tot[h][2]);
+      tot[h][3] = fmaf(acc[h][3], sc[2 * h + 1], tot[h][3]);
     }
     int4 job = make_int4(0, 0, 0, 0);
     if (meta < 0) job = ct.job[st];
@@ -701,16 +614,20 @@ int gl_launch_gmm_w4(const void* x, const void* w4, const float* s, const int32_
     return -1;
   }
   // 32 columns x words x strips of 32 columns: a box is 16 strips of 16 words
-  CUtensorMap wmap;
+  CUtensorMap wmap, xmap;
   if (!gl_make_tmap_3d(&wmap, CU_TENSOR_MAP_DATA_TYPE_INT32, w4, 32, G * (K / 8), N / 32, N, 32, 32, 16,
                        COLS / 32, CU_TENSOR_MAP_SWIZZLE_128B, why))
     return -1;
+  // 64 features x rows x 64-feature pieces: a box is two pieces of 8 rows
+  if (!gl_make_tmap_3d(&xmap, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, 64, M, K / 64, K, 64, 64, ROWS, 2,
+                       CU_TENSOR_MAP_SWIZZLE_128B, why))
+    return -1;
   unsigned long long* tags = static_cast<unsigned long long*>(ws);
   float* parts = reinterpret_cast<float*>(tags + n * WARPS);
-  const Args a{static_cast<const uint4*>(x), s, group_sizes, tags, parts, next_nonce(), M, N,
+  const Args a{s, group_sizes, tags, parts, next_nonce(), M, N,
                static_cast<int>(G), kb, static_cast<int>(strips), out, out_f32, zero_tail, err};
   if (!gl_set_smem_attr(reinterpret_cast<const void*>(&gmm_w4_kernel), 0, SMEM_BYTES, why)) return -2;
-  gl::launch_following(gmm_w4_kernel, n, THREADS, SMEM_BYTES, st, wmap, a);
+  gl::launch_following(gmm_w4_kernel, n, THREADS, SMEM_BYTES, st, wmap, xmap, a);
   return launched(why);
 }
 

@@ -203,6 +203,61 @@ def test_graph_replays_share_nothing(cuda):
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+def _weighs_only_what_it_meets(out, x, q, s, sizes):
+    """_check with |q| for |q| + 16: an x whose weight is 0 adds nothing, also no error."""
+    row, K = 0, x.shape[1]
+    for g, n in enumerate(sizes):
+        sc = s[g].to(F64).repeat_interleave(128, 0)
+        xr = x[row:row + n].to(F64)
+        ref, mag = xr @ (q[g].to(F64) * sc), xr.abs() @ (q[g].abs().to(F64) * sc)
+        tol = (8 * 2.0 ** -22 + (K / 128 + 16) * 2.0 ** -24) * mag
+        err = (out[row:row + n].to(F64) - ref).abs()
+        assert (err <= tol).all(), (g, float((err / mag).max()))
+        row += n
+
+
+@pytest.mark.parametrize("large", [1e2, 1e4, 1e6, 1e20, 1e38])
+@pytest.mark.parametrize("K,N,sizes", [(128, 32, [1]), (1024, 96, [3, 0, 9]), (7168, 512, [1])])
+def test_large_x_against_weights_of_zero(cuda, K, N, sizes, large):
+    # outliers in some features, as in front of a down projection: their weights
+    # are 0 in every column, so the output is that of the other features
+    w4, s = _weights(cuda, len(sizes), K, N, seed=15)
+    at = torch.arange(0, K, 37, device=cuda)
+    for k in at.tolist():
+        word, bit = w4[:, k // 8], 4 * (k % 8)
+        eight = 8 << bit
+        w4[:, k // 8] = (word & ~torch.tensor(15 << bit, device=cuda).to(torch.int32)) | \
+            torch.tensor(eight - 2 ** 32 if eight >= 2 ** 31 else eight, device=cuda).to(torch.int32)
+    q = _unpack(w4)
+    assert (q[:, at] == 0).all()
+    x = _x(cuda, sum(sizes), K, seed=16)
+    gs = torch.tensor(sizes, dtype=torch.int32, device=cuda)
+    x[:, at] = (x[:, at].float().sign() * large).to(BF16)
+    out = ops.gmm_w4_fwd(x, w4, s, gs)
+    _weighs_only_what_it_meets(out, x, q, s, sizes)
+    x[:, at] = 0
+    assert torch.equal(ops.gmm_w4_fwd(x, w4, s, gs), out)
+    assert ops.device_status() == 0
+
+
+def test_small_x_beside_large_ones(cuda):
+    # a column reads features 2^-20 to 2^-45 of the block's largest: every one in full
+    K, N = 128, 32
+    x = torch.full((8, K), 3.0, device=cuda)
+    small = (1 + torch.arange(8, device=cuda) / 128) * 2.0 ** -torch.arange(20, 52, 4, device=cuda)
+    x[:, 40:48] = small
+    x = x.to(BF16)
+    q = torch.zeros((K, N), dtype=torch.int64, device=cuda)
+    q[40:48] = torch.eye(8, dtype=torch.int64, device=cuda).repeat(1, 4) * 5  # column n reads feature 40 + n % 8
+    word = torch.zeros((K // 8, N), dtype=torch.int64, device=cuda)
+    for j in range(8):
+        word |= (q[j::8] + 8) << (4 * j)
+    w4 = torch.where(word >= 2 ** 31, word - 2 ** 32, word).to(torch.int32)[None].contiguous()
+    out = ops.gmm_w4_fwd(x, w4, torch.ones((1, 1, N), device=cuda), torch.tensor([8], dtype=torch.int32, device=cuda))
+    want = x[:, 40:48].float().repeat(1, 4) * 5
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("K,N,sizes", [(14336, 512, [1]), (7168, 512, [8]), (7168, 1024, [3, 0, 2, 5])])
 def test_jobs_of_many_ctas_are_the_same_every_time(cuda, K, N, sizes):
     # every tile's k is cut among CTAs, and whichever of them is last adds all parts
