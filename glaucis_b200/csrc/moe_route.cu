@@ -184,26 +184,59 @@ __device__ __forceinline__ bool takes_part(const float (&z)[V]) {
   return __any_sync(FULL, any);
 }
 
-// e^x for x <= 0 as 2^(x log2 e): two roundings of the exponent, |x| 2^-24
-// relative each, where subtracting the row's maximum already made one.  Results
-// below 2^-126 of the largest numerator are 0.
-__device__ __forceinline__ float exp_of(float x) {
+// e^x for x <= 0 as 2^t (1 + d ln 2), t = x log2 e rounded and d what that rounding
+// and the constant's own left out: within 2 ulp at every x, where 2^t alone is off
+// by |x| 2^-24 relative.  Results below 2^-126 are 0; -inf, whose d has no value,
+// is held at -200, and NaN goes through.  (32768 tokens of 128 experts, forward
+// and gradient: 39.1 us, 38.1 with 2^t alone, 40.4 with expf.)
+constexpr float LOG2E = 1.44269504f, LOG2E_LOW = 1.92596299e-8f;  // 24 bits and the next ones
+constexpr float LN2 = 0.693147181f;
+
+__device__ __forceinline__ float bounded(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-200.0f));
+  return x;
+}
+
+__device__ __forceinline__ float exp2_of(float t) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
+}
+
+__device__ __forceinline__ float exp_of(float x) {
+  x = bounded(x);
+  const float t = x * LOG2E, r = exp2_of(t);
+  return fmaf(r, fmaf(x, LOG2E_LOW, fmaf(x, LOG2E, -t)) * LN2, r);
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Two at once on packed f32x2 arithmetic.
+__device__ __forceinline__ float2 exp_of(float2 x) {
+  x = make_float2(bounded(x.x), bounded(x.y));
+  const float2 nt = __fmul2_rn(x, both(-LOG2E));
+  const float2 r = make_float2(exp2_of(-nt.x), exp2_of(-nt.y));
+  const float2 d = __ffma2_rn(x, both(LOG2E_LOW), __ffma2_rn(x, both(LOG2E), nt));
+  return __ffma2_rn(r, __fmul2_rn(d, both(LN2)), r);
 }
 
 // Softmax numerators e of the logits z (0 where z is -inf and zmax is not);
 // returns 1 / their sum.
 template <int V>
 __device__ __forceinline__ float softmax(const float (&z)[V], float zmax, float (&e)[V]) {
-  float s = 0.0f;
+  float2 s = both(0.0f);
+  if constexpr (V == 1) {
+    s.x = e[0] = exp_of(z[0] - zmax);
+  } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    e[i] = exp_of(z[i] - zmax);
-    s += e[i];
+    for (int i = 0; i < V; i += 2) {
+      const float2 v = exp_of(__fadd2_rn(make_float2(z[i], z[i + 1]), both(-zmax)));
+      s = __fadd2_rn(s, v);
+      e[i] = v.x;
+      e[i + 1] = v.y;
+    }
   }
-  return __fdividef(1.0f, warp_sum(s));  // the sum is 1 to 1024: within 2 ulp
+  return __fdividef(1.0f, warp_sum(s.x + s.y));  // the sum is 1 to 1024: within 2 ulp
 }
 
 // A lane's keys and where they are, so that the largest is at hand and the next
@@ -493,7 +526,7 @@ __device__ void finish(const Args& a, Sh& sh, int rows, int n) {
 
 // One CTA takes every token.
 template <int V>
-__global__ void __launch_bounds__(32 * warps<V>()) route_one_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * warps<V>(), 1) route_one_kernel(const Args a) {
   __shared__ RouteShared<V> sh;
   follow();
   route_tokens<V, true>(a, 0, a.T, sh);
@@ -617,8 +650,10 @@ __device__ __forceinline__ void store_token(const Args& a, void* out, int64_t t,
 // the gradient d of the chosen experts' weights w plus w_e (d_e - sum_e' w_e' d_e')
 // on those, or, where w is p as it is, p_e d_e there less p_e sum_e' p_e' d_e'
 // everywhere.
+// Five CTAs an SM with up to two experts a lane: 22.1 us for 65536 tokens of 64, 24.4
+// with the four that its registers would leave.
 template <int V>
-__global__ void __launch_bounds__(256) route_bwd_kernel(const Args a, const BwdArgs b) {
+__global__ void __launch_bounds__(256, V <= 2 ? 5 : 0) route_bwd_kernel(const Args a, const BwdArgs b) {
   const int lane = threadIdx.x & 31;
   // a token's logits and choices, read one token ahead
   float next[V], w_next = 0.0f, sel_next = 0.0f;

@@ -105,6 +105,38 @@ def test_mask_and_what_padding_holds(cuda, T, E, k):
     assert (r.ids[~mask] == -1).all() and (r.pos[~mask] == -1).all() and (r.weights[~mask] == 0).all()
 
 
+@pytest.mark.parametrize("E", [1, 7, 32, 60, 128, 256, 500, 1024])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_small_probabilities_keep_their_bits(cuda, E, bf16):
+    # whole logits: subtracting the largest is exact, so a probability is off by
+    # 2 ulp of the exponential (4 u) above and in the sum, by (E / 32 + 5) u of
+    # the sum itself, 4 u of its reciprocal and u of the product, whatever its
+    # size; and the loss as in _check_forward, without the subtraction's share.
+    k, T = min(E, 8), 300
+    g = torch.Generator(device=cuda).manual_seed(E)
+    z = -torch.randint(0, 87, (T, E), generator=g, device=cuda).float()
+    z[1] = -80
+    z[1, 0] = 0
+    z = z.to(torch.bfloat16) if bf16 else z
+    r = ops.moe_route_fwd(z, k, renormalize=False)
+    ref = _reference(z, k, None, False)
+    tol = (E / 32 + 18) * U
+    assert np.array_equal(r.ids.cpu().numpy(), ref["ids"])
+    err = np.abs(r.weights.double().cpu().numpy() - ref["w"])
+    assert (err <= tol * ref["w"]).all(), float((err / ref["w"]).max() / U)
+    assert abs(float(r.balance_loss) - ref["loss"]) <= (tol + (T / 32 + 32 + 148 + 10) * U) * ref["loss"]
+    # the gradient of the loss alone: p (c - sum p c), every p and the sum so
+    dl = ops.moe_route_bwd(z, r, None, torch.ones((), device=cuda)).double().cpu().numpy()
+    c = E * ref["f"] / ref["n"]
+    mean = (ref["p"] * c).sum(1, keepdims=True)
+    want = ref["p"] * (c - mean)
+    bound = ref["p"] * (tol * np.abs(c - mean) + (2 * tol + (E / 32 + 12) * U) * (np.abs(c) + mean))
+    # its rounding: half a step, of the type's subnormals 2^-133 (bf16) or of a
+    # few products that end at 2^-149 (fp32)
+    half = 2.0 ** -8 * np.abs(want) + 2.0 ** -134 if bf16 else U * np.abs(want)
+    assert (np.abs(dl - want) <= bound + half + 8 * 2.0 ** -149).all()
+
+
 def test_ties_go_to_the_lowest_expert(cuda):
     logits = torch.zeros((40, 128), device=cuda)
     logits[1::2] = -0.0
