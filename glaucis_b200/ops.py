@@ -865,8 +865,12 @@ def moe_route_bwd(logits: torch.Tensor, routing: MoERouting, dweights: Optional[
     with _same_device(logits, r.ids, r.weights, r.counts, r.routed, r.mask, dweights, dloss):
         T, E = _route_check(logits, r.mask)
         topk = r.ids.shape[1]
-        if tuple(r.ids.shape) != (T, topk) or r.weights.shape != r.ids.shape or r.counts.numel() != E:
+        if tuple(r.ids.shape) != (T, topk) or r.weights.shape != r.ids.shape or r.counts.numel() != E \
+                or r.routed.numel() != 1:
             raise ValueError("routing does not belong to these logits")
+        if r.ids.dtype != torch.int32 or r.counts.dtype != torch.int32 or r.weights.dtype != torch.float32 \
+                or r.routed.dtype != torch.float32:
+            raise ValueError("routing's tensors must have the types that belong to moe_route_fwd's")
         if dweights is not None and (dweights.dtype != torch.float32 or dweights.shape != r.ids.shape):
             raise ValueError("dweights must be fp32 [T, topk]")
         if dloss is not None and (dloss.dtype != torch.float32 or dloss.numel() != 1):

@@ -314,6 +314,17 @@ def test_offsets_past_32_bits(cuda):
     assert torch.isfinite(dl[-500:].float()).all()
 
 
+def test_backward_refuses_another_routings_types(cuda):
+    z = torch.zeros((4, 16), device=cuda)
+    r = ops.moe_route_fwd(z, 2)
+    dw = torch.zeros((4, 2), device=cuda)
+    for bad in (dict(ids=r.ids.long()), dict(counts=r.counts.long()), dict(weights=r.weights.double()),
+                dict(routed=r.routed.double()), dict(routed=r.routed.expand(2).contiguous()),
+                dict(counts=r.counts[:8].contiguous())):
+        with pytest.raises(ValueError, match="belong"):
+            ops.moe_route_bwd(z, r._replace(**bad), dw, None)
+
+
 def test_refusals(cuda):
     z = torch.zeros((4, 16), device=cuda)
     for bad in (z.half(), z[0], z.double()):
