@@ -314,6 +314,25 @@ def test_offsets_past_32_bits(cuda):
     assert torch.isfinite(dl[-500:].float()).all()
 
 
+def test_gradient_past_32_bits_is_that_of_its_rows(cuda):
+    # the last tokens' logits lie past 2^31 elements and 2^32 bytes; without the
+    # loss a token's gradient depends on its own row alone
+    T, E, k, n = 2_200_000, 1024, 4, 500
+    logits = torch.zeros((T, E), dtype=torch.bfloat16, device=cuda)
+    logits[:, 3:7] = 1
+    logits[-n:] = _logits(cuda, n, E, True, seed=31)
+    dw = torch.randn((T, k), generator=torch.Generator(device=cuda).manual_seed(32), device=cuda)
+    for renorm in (True, False):
+        r = ops.moe_route_fwd(logits, k, renormalize=renorm)
+        dl = ops.moe_route_bwd(logits, r, dw, None)
+        tail = logits[-n:].clone()
+        rt = ops.moe_route_fwd(tail, k, renormalize=renorm)
+        want = ops.moe_route_bwd(tail, rt, dw[-n:].contiguous(), None)
+        assert want.float().abs().amax(1).min() > 0
+        assert torch.equal(dl[-n:], want)
+        del dl, r
+
+
 def test_backward_refuses_another_routings_types(cuda):
     z = torch.zeros((4, 16), device=cuda)
     r = ops.moe_route_fwd(z, 2)
