@@ -12,6 +12,7 @@ import contextlib
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -663,6 +664,40 @@ def _new_like(like: torch.Tensor, t: Optional[torch.Tensor], dtype: torch.dtype,
     return torch.empty_like(like, dtype=dtype)
 
 
+def _records(name: str, *ts: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records this call of `name`.  A tensor that carries a
+    forward-mode tangent is refused: no operator here has one for its outputs."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual_level
+        for t in ts:
+            if t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+class _NoGradient(torch.autograd.Function):
+    """A call without a backward inside a recorded computation: its gradient is
+    an error when it is asked for, not missing."""
+    @staticmethod
+    def forward(ctx, name, call, args, *inputs):
+        ctx.name = name
+        return call(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no gradient: detach its inputs or call it under torch.no_grad()")
+
+
+def _without_gradient(name: str, call, args, outs, *inputs: Optional[torch.Tensor]):
+    """call(*args), recorded as _NoGradient of the inputs."""
+    if any(o is not None for o in outs):
+        raise RuntimeError(f"{name} has no gradient and takes preallocated outputs under torch.no_grad() only")
+    return _NoGradient.apply(name, call, args, *inputs)
+
+
 class RMSNormForward(NamedTuple):
     """Result of rms_norm_fwd.  y (bf16) and q, s (e4m3 and its 1x128 scales)
     are None unless asked for; h is the stored sum (x itself without a
@@ -706,8 +741,16 @@ def rms_norm_quant_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-
 
     The layout and scales are quant_act_1x128's; the norm enters them in 32
     bits, so the pair is rounded once.  q, s and h may be given preallocated;
-    h may be `x` or `residual` itself.
+    h may be `x` or `residual` itself.  It has no gradient (rms_norm has):
+    asking for one of its outputs is an error.
     """
+    if _records("rms_norm_quant_1x128", x, weight, residual):
+        return _without_gradient("rms_norm_quant_1x128", _rms_norm_quant_1x128, (x, weight, eps, residual, q, s, h),
+                                 (q, s, h), x, weight, residual)
+    return _rms_norm_quant_1x128(x, weight, eps, residual, q, s, h)
+
+
+def _rms_norm_quant_1x128(x, weight, eps, residual, q, s, h):
     with _same_device(x, weight, residual):
         M, K = _rms_check(x, weight, residual)
         if h is not None and residual is None:
@@ -791,7 +834,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
              residual: Optional[torch.Tensor] = None):
     """RMS norm in bf16, differentiable in x, weight and residual: y, or with a
     residual (y, h), h = bf16(x + residual) being the stream that goes on."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _records("rms_norm", x, weight, residual):
         return _RMSNorm.apply(x, weight, eps, residual)
     f = rms_norm_fwd(x, weight, eps, residual=residual)
     return f.y if residual is None else (f.y, f.h)
@@ -908,7 +951,7 @@ class _MoERoute(torch.autograd.Function):
 def moe_route(logits: torch.Tensor, topk: int, *, mask: Optional[torch.Tensor] = None,
               renormalize: bool = True) -> MoERouting:
     """moe_route_fwd, its weights and balance loss differentiable in logits."""
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _records("moe_route", logits):
         out = _MoERoute.apply(logits, topk, mask, renormalize)
         return MoERouting(*out, mask, renormalize)
     return moe_route_fwd(logits, topk, mask=mask, renormalize=renormalize)
@@ -953,7 +996,15 @@ def moe_dispatch_quant(q: torch.Tensor, s: torch.Tensor, pos: torch.Tensor, grou
     """moe_dispatch of quantised rows: q e4m3 [T, K] and s fp32 [T, K/128]
     (quant_act_1x128 or rms_norm_quant_1x128 of the tokens) -> the operands of
     gmm_fp8_fwd, quantised once per token instead of once per choice.  Rows
-    past sum(group_sizes) are zeros with scale 1."""
+    past sum(group_sizes) are zeros with scale 1.  It has no gradient: asking
+    for one of its outputs is an error."""
+    if _records("moe_dispatch_quant", q, s):
+        return _without_gradient("moe_dispatch_quant", _moe_dispatch_quant,
+                                 (q, s, pos, group_sizes, rows, out, out_s), (out, out_s), q, s)
+    return _moe_dispatch_quant(q, s, pos, group_sizes, rows, out, out_s)
+
+
+def _moe_dispatch_quant(q, s, pos, group_sizes, rows, out, out_s):
     with _same_device(q, s, pos, group_sizes):
         T, topk = _pos_check(pos, group_sizes)
         if q.dtype != FP8 or q.dim() != 2 or q.shape[0] != T:
@@ -1006,7 +1057,7 @@ def moe_dispatch(x: torch.Tensor, pos: torch.Tensor, group_sizes: torch.Tensor,
     one choice; a negative one is skipped); the lhs of gmm_fp8_blockwise with group_sizes =
     counts.  `rows` (default T * topk) is the number of output rows; those past
     sum(group_sizes) are zero.  Differentiable in x (bf16)."""
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _records("moe_dispatch", x):
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] > 16384:
             raise ValueError("the differentiable moe_dispatch takes bf16 [T, K], K at most 16384")
         return _MoEDispatch.apply(x, pos, group_sizes, rows)
@@ -1079,7 +1130,7 @@ def moe_combine(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, group
     weights[t, j] * y[pos[t, j]] (y bf16 or fp32 [rows, K], out bf16), summed in
     fp32 and rounded once; for pos, weights and counts (group_sizes) of
     moe_route.  Differentiable in y, weights and residual."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, residual)):
+    if _records("moe_combine", y, weights, residual):
         return _MoECombine.apply(y, pos, weights, group_sizes, residual)
     return moe_combine_fwd(y, pos, weights, residual=residual)
 
@@ -1109,9 +1160,15 @@ def gmm_w4_fwd(x: torch.Tensor, w4: torch.Tensor, s: torch.Tensor, group_sizes: 
     """Grouped matmul of few rows with 4-bit weights: x bf16 [M, K] (rows in
     group order), w4 and s as quant_w4_128x1 gives them, group_sizes int32 [G]
     -> [M, N].  The decoding counterpart of gmm_fp8_fwd: reads half a byte a
-    weight of the groups that have rows, and x in bf16.  The weights are not
-    differentiated.  Rows at or beyond sum(group_sizes) are left as they are in
+    weight of the groups that have rows, and x in bf16.  It has no gradient:
+    asking for one of its output is an error.  Rows at or beyond sum(group_sizes) are left as they are in
     `out` (zeroed when allocated)."""
+    if _records("gmm_w4_fwd", x, s):
+        return _without_gradient("gmm_w4_fwd", _gmm_w4, (x, w4, s, group_sizes, out_dtype, out), (out,), x, s)
+    return _gmm_w4(x, w4, s, group_sizes, out_dtype, out)
+
+
+def _gmm_w4(x, w4, s, group_sizes, out_dtype, out):
     with _same_device(x, w4, s, group_sizes, out):
         if x.dtype != torch.bfloat16 or x.dim() != 2:
             raise ValueError("x must be a 2-D bf16 tensor")

@@ -371,3 +371,70 @@ def test_norm_and_router_see_the_call_before(cuda, T, K):
         graph.replay()
         assert torch.equal(got, ids) and torch.equal(b["h"], want)
     assert ops.device_status() == 0
+
+
+def _one_expert(cuda, T=4, K=256, N=64):
+    g = torch.Generator(device=cuda).manual_seed(40)
+    x = torch.randn((T, K), generator=g, device=cuda).to(torch.bfloat16)
+    w4 = torch.randint(-2 ** 31, 2 ** 31, (1, K // 8, N), generator=g, device=cuda, dtype=torch.int32)
+    return x, w4, torch.ones((1, K // 128, N), device=cuda), torch.tensor([T], dtype=torch.int32, device=cuda)
+
+
+def test_a_gradient_that_does_not_exist_is_an_error(cuda):
+    # a call that takes part in a recorded computation but has no backward says
+    # so when the gradient is asked for; without one it runs as ever
+    x, w4, s, sizes = _one_expert(cuda)
+    w = torch.ones(x.shape[1], device=cuda)
+    pos = torch.arange(4, dtype=torch.int32, device=cuda)[:, None].contiguous()
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    clean = ops.gmm_w4_fwd(x, w4, s, sizes)
+    out = ops.gmm_w4_fwd(xg, w4, s, sizes)
+    assert torch.equal(out, clean) and not clean.requires_grad
+    with pytest.raises(RuntimeError, match="gmm_w4_fwd"):
+        out.sum().backward()
+    q, sc = ops.quant_act_1x128(x)
+    scg = sc.clone().requires_grad_()
+    _, moved = ops.moe_dispatch_quant(q, scg, pos, sizes)
+    assert torch.equal(moved, sc)
+    with pytest.raises(RuntimeError, match="moe_dispatch_quant"):
+        moved.sum().backward()
+    for a, b in ((xg, w), (x, wg)):
+        pair = ops.rms_norm_quant_1x128(a, b, residual=x)
+        with pytest.raises(RuntimeError, match="rms_norm_quant_1x128"):
+            pair[2].float().sum().backward()
+    assert xg.grad is None and wg.grad is None
+    # a given output cannot carry that: refused where a gradient is recorded
+    own = torch.empty_like(clean)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        ops.gmm_w4_fwd(xg, w4, s, sizes, out=own)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        ops.rms_norm_quant_1x128(xg, w, residual=x, h=torch.empty_like(x))
+    with pytest.raises(RuntimeError, match="no_grad"):
+        ops.moe_dispatch_quant(q, scg, pos, sizes, out_s=torch.empty_like(sc))
+    with torch.no_grad():
+        assert torch.equal(ops.gmm_w4_fwd(xg, w4, s, sizes, out=own), clean)
+        assert not ops.rms_norm_quant_1x128(xg, wg)[1].requires_grad
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    from torch.autograd import forward_ad as fw
+    x, w4, s, sizes = _one_expert(cuda)
+    w = torch.ones(x.shape[1], device=cuda)
+    pos = torch.arange(4, dtype=torch.int32, device=cuda)[:, None].contiguous()
+    one = torch.ones((4, 1), device=cuda)
+    q, sc = ops.quant_act_1x128(x)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for name, call in [("rms_norm", lambda: ops.rms_norm(dual(x), w)),
+                           ("rms_norm", lambda: ops.rms_norm(x, w, residual=dual(x))),
+                           ("rms_norm_quant_1x128", lambda: ops.rms_norm_quant_1x128(x, dual(w))),
+                           ("moe_route", lambda: ops.moe_route(dual(x[:, :8].float().contiguous()), 2)),
+                           ("moe_dispatch", lambda: ops.moe_dispatch(dual(x), pos, sizes)),
+                           ("moe_dispatch_quant", lambda: ops.moe_dispatch_quant(q, dual(sc), pos, sizes)),
+                           ("moe_combine", lambda: ops.moe_combine(x, pos, dual(one), sizes)),
+                           ("gmm_w4_fwd", lambda: ops.gmm_w4_fwd(dual(x), w4, s, sizes))]:
+            with pytest.raises(RuntimeError, match=f"{name}.*forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name}.*forward-mode"):
+                call()
+        assert torch.equal(ops.rms_norm(x, w), ops.rms_norm_fwd(x, w).y)  # no tangent, no refusal
