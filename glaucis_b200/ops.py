@@ -1131,6 +1131,11 @@ def moe_combine(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor, group
     fp32 and rounded once; for pos, weights and counts (group_sizes) of
     moe_route.  Differentiable in y, weights and residual."""
     if _records("moe_combine", y, weights, residual):
+        # what the backward alone reads
+        _same_device(y, group_sizes)
+        _pos_check(pos, group_sizes)
+        if not 1 <= group_sizes.numel() <= 1024:
+            raise ValueError("the differentiable moe_combine takes group_sizes of 1 to 1024 groups")
         return _MoECombine.apply(y, pos, weights, group_sizes, residual)
     return moe_combine_fwd(y, pos, weights, residual=residual)
 

@@ -438,3 +438,19 @@ def test_forward_mode_tangents_are_refused(cuda):
             with torch.no_grad(), pytest.raises(RuntimeError, match=f"{name}.*forward-mode"):
                 call()
         assert torch.equal(ops.rms_norm(x, w), ops.rms_norm_fwd(x, w).y)  # no tangent, no refusal
+
+
+def test_combine_refuses_early_what_its_gradient_could_not_take(cuda):
+    T, K = 4, 64
+    y = torch.ones((T, K), device=cuda, requires_grad=True)
+    pos = torch.arange(T, dtype=torch.int32, device=cuda)[:, None].contiguous()
+    w = torch.ones((T, 1), device=cuda)
+    sizes = torch.tensor([T], dtype=torch.int32, device=cuda)
+    for bad in (sizes.long(), sizes.cpu(), sizes[None], torch.zeros(1025, dtype=torch.int32, device=cuda),
+                torch.zeros(0, dtype=torch.int32, device=cuda)):
+        with pytest.raises(ValueError, match="group_sizes|CUDA"):
+            ops.moe_combine(y, pos, w, bad)
+        with pytest.raises(ValueError, match="group_sizes|CUDA"):
+            ops.moe_combine(y.detach(), pos, w.clone().requires_grad_(), bad)
+    ops.moe_combine(y, pos, w, sizes).sum().backward()
+    assert (y.grad == 1).all()
