@@ -3,6 +3,10 @@ current stream, allocate nothing in the library, and the GLA sequence split
 forks its library-owned side stream from, and joins it back to, the
 capturing stream with events.  A replay must reproduce the eager result bit
 for bit."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -62,3 +66,23 @@ def test_gla_forward_replays_bit_for_bit(cuda, B, T, H):
     torch.cuda.synchronize()
     assert ops.device_status() == 0
     assert torch.equal(o, want_o) and torch.equal(ht, want_ht)
+
+
+def test_the_launch_stream_is_the_current_one(cuda):
+    # the raw handle that the ops launch on, against the public object's
+    side = torch.cuda.Stream()
+    assert ops._stream() == torch.cuda.current_stream().cuda_stream
+    with torch.cuda.stream(side):
+        assert ops._stream() == side.cuda_stream == torch.cuda.current_stream().cuda_stream
+        assert ops.device_status() == 0
+    assert ops._stream() == torch.cuda.current_stream().cuda_stream != side.cuda_stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert ops._stream() == torch.cuda.current_stream().cuda_stream
+
+
+def test_status_before_anything_else_of_a_process(cuda):
+    # neither a tensor nor a stream exists yet
+    code = "from glaucis_b200 import ops; assert ops.device_status() == 0"
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], cwd=root, check=True, timeout=300)
