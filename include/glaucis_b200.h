@@ -402,7 +402,8 @@ int gl_moe_route_bwd(const void* logits, int logits_f32, const void* mask, const
 /*
  * Rows into expert order: out[pos[t, j]] = x[t] for every pos >= 0.
  *   x            [T, row_bytes] (any type; row_bytes a multiple of 16)
- *   s            fp32 [T, scales] moved alongside into out_s, or both NULL
+ *   s            fp32 [T, scales] moved alongside into out_s, or both NULL and
+ *                scales 0 (with scales and T == 0, s may be NULL)
  *   pos          int32 [T, topk] as gl_moe_route_fwd writes it: the rows below
  *                sum(group_sizes), each of one choice (one that no choice names
  *                is left as it is); a negative one is skipped
@@ -463,13 +464,16 @@ int gl_quant_w4_128x1(const void* w, int64_t G, int64_t K, int64_t N, void* w4, 
  *       checkpoint's own scales will do);  group_sizes int32 [G] (device)
  *   out [M, N] bf16 or fp32 (out_dtype); rows at or past sum(group_sizes) are
  *       left as they are, or zeroed with GL_W4_ZERO_TAIL
- * Products are exact, sums fp32.  A non-finite x makes its row's outputs
- * non-finite.  K % 128 == 0, N % 32 == 0, 1 <= G <= 1024, M <= 65536; x, w4, s,
- * out and the workspace 16-byte aligned.  The weights of a group are read once per 32
- * rows of it: gl_gmm_fp8_fwd is the better choice for many rows.
- * workspace: gl_gmm_w4_workspace_bytes(M, K) bytes on the current device (0
- * for an unsupported shape or M == 0), not used by another call in flight.  Negative sizes or a sum past M
- * set GL_DEV_BAD_GROUPS (out is then unspecified).
+ * Products are exact, sums fp32 (finite while those of |x q| over a block of 128
+ * k stay below 2^134).  A non-finite x makes its row's outputs non-finite.
+ * K % 128 == 0, N % 32 == 0, 1 <= G <= 1024, M <= 65536; x, w4, s, out and the
+ * workspace 16-byte aligned.  The weights of a group are read once for every 8
+ * rows of it: from about 16 rows a group on gl_gmm_fp8_fwd is the better choice.
+ * workspace: gl_gmm_w4_workspace_bytes(M, K) bytes on the current device (0 for
+ * an unsupported shape or M == 0), not used by another call in flight; what it
+ * holds before does not matter, but for a captured call that ended with
+ * GL_DEV_WAIT_TIMEOUT: clear it before that graph is replayed.  Negative sizes or
+ * a sum past M set GL_DEV_BAD_GROUPS (out is then unspecified).
  */
 size_t gl_gmm_w4_workspace_bytes(int64_t M, int64_t K);
 int gl_gmm_w4_fwd(const void* x, const void* w4, const float* s, const int32_t* group_sizes, int64_t G,
