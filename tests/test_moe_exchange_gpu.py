@@ -218,6 +218,30 @@ def test_no_tokens_but_rows_of_a_capacity(cuda):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("T", [1, 3])
+def test_few_tokens_in_rows_of_a_capacity(cuda, T):
+    # more rows than the choices can fill: the rest is zero, its scales 1
+    E, k, K, rows = 8, 2, 512, 5000
+    pos, sizes = _routing(cuda, T, E, k, seed=50)
+    g = torch.Generator(device=cuda).manual_seed(51)
+    x = torch.randn((T, K), generator=g, device=cuda).to(BF16)
+    named = pos.reshape(-1).long()
+    junk = lambda *s, dtype=BF16: torch.full(s, float("nan"), device=cuda).to(dtype)  # noqa: E731
+    out = ops.moe_dispatch_fwd(x, pos, sizes, rows, junk(rows, K))
+    assert torch.equal(out[named], x.repeat_interleave(k, 0)) and (out[T * k:] == 0).all()
+    q, s = ops.quant_act_1x128(x)
+    oq, os_ = ops.moe_dispatch_quant(q, s, pos, sizes, rows, junk(rows, K, dtype=E4M3), junk(rows, K // 128, dtype=F32))
+    assert torch.equal(os_[named], s.repeat_interleave(k, 0)) and (os_[T * k:] == 1).all()
+    assert torch.equal(oq[named].view(torch.uint8), q.view(torch.uint8).repeat_interleave(k, 0))
+    assert (oq[T * k:].float() == 0).all()
+    y = torch.randn((rows, K), generator=g, device=cuda).to(BF16)
+    w = torch.rand((T, k), generator=g, device=cuda)
+    dy, dw = ops.moe_combine_bwd(x, y, pos, w, sizes)
+    assert (dy[T * k:] == 0).all()
+    assert torch.equal(dy[named], (w.reshape(-1, 1) * x.float().repeat_interleave(k, 0)).to(BF16))
+    assert ops.device_status() == 0
+
+
 def test_refusals(cuda):
     T, K = 4, 256
     x, pos = _rand(cuda, T, K), torch.zeros((T, 2), dtype=torch.int32, device=cuda)
