@@ -483,7 +483,7 @@ __device__ __forceinline__ float2 markstein2(float2 nx, float2 ny, float2 s) {
 // coherent with what the other kernel still wrote when this one had started:
 // fetch() instead.  For kernels that follow one another without work of the
 // host's between them: us a call in a stream, against plain launches, one token's
-// 4-bit product 17.4 (18.9), rows out and back with gradients 308 (321).  Kernels
+// 4-bit product 18.1 (20.7), rows out and back with gradients 308 (321).  Kernels
 // that gained nothing, the norm's backward and the larger routers, start plainly.
 // The next kernel launched so may start from the CTAs' call of may_follow() on,
 // by default made at once; it waits in its follow() likewise.

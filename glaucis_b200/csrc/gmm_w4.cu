@@ -32,8 +32,9 @@
 //     of 1e-6.
 // Sums stay in fp32's range while those of |q x| in a block stay below 2^134.
 // Measured in a CUDA graph (K 7168, N 2048, 128 groups): 128 rows in 44 groups 67
-// us, 5.2 TB/s of weights and scales (64 us without finishing split jobs, 54.5 us
-// without the sums too); 8 rows in 8 groups 17.9 us (15.7, 11.9).
+// us, 5.1 TB/s of weights and scales (64 us without finishing split jobs, 54.5 us
+// without the sums too), 74 at the power cap of a loop; 8 rows in 8 groups 17.9 us
+// (15.7, 11.9).
 #include "common.cuh"
 
 #include <atomic>

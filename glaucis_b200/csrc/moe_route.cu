@@ -11,7 +11,7 @@
 // Each lane keeps the largest of its own keys at hand, so a round is one
 // redux.max for the key, a redux.min for the lowest expert that has it, and the
 // winner's next key taking its place.  With E floats a token to read it is bound
-// by issuing these instructions, mostly integer ones (440 a token of 128 experts
+// by issuing these instructions, mostly integer ones (460 a token of 128 experts
 // and 8 choices), not by HBM.
 //
 // Rows need the counts of all earlier tokens: each CTA takes consecutive tokens
@@ -20,9 +20,9 @@
 // in order.  Counts are integers and the loss's sums run in a fixed order over
 // warps and CTAs: results do not depend on timing.
 //
-// Measured, 128 experts, top 8: 3 tokens 4.0 us, 4096 9.7 us, 32771 with the
-// gradient 37 us; 32768 tokens of 256 experts 36 us, 16384 of 384 41 us, 8192 of
-// 1024 68 us.
+// Measured in a CUDA graph, 128 experts, top 8: 3 tokens 4.0 us, 4096 10 us, 32771
+// with the gradient 39 us; 32768 tokens of 256 experts 37 us, 16384 of 384 42 us,
+// 8192 of 1024 69 us.
 #include "common.cuh"
 
 #include <atomic>
